@@ -39,11 +39,27 @@ def sources():
 
 
 def headers():
-    return sorted(glob.glob(os.path.join(HERE, "*.hpp")) + glob.glob(os.path.join(HERE, "*.inc")) + glob.glob(os.path.join(HERE, "..", "..", "include", "*.h")))
+    return sorted(glob.glob(os.path.join(HERE, "*.hpp")) + glob.glob(os.path.join(HERE, "*.inc")) + [os.path.join(HERE, "..", "..", "include", "geneface_hip.h")])
+
+
+# The operators of a training step (train/: AdamW, block-scaled 8-bit products) are translation units of the same library with a public header of
+# their own.  Nothing above includes from there and they include only common.hpp, so neither side's edits rebuild the other, and the digest
+# below, which stamps measurements of the frame and field kernels, does not move with them.  They are compiled without the packed-FP32 feature:
+# the same ban as -fno-slp-vectorize for code that is written on vectors.
+TRAIN_DIR = os.path.join(HERE, "train")
+TRAIN_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option"]
+
+
+def train_sources():
+    return sorted(glob.glob(os.path.join(TRAIN_DIR, "*.hip")))
+
+
+def train_headers():
+    return sorted(glob.glob(os.path.join(TRAIN_DIR, "*.hpp")) + [os.path.join(HERE, "common.hpp"), os.path.join(HERE, "..", "..", "include", "geneface_train_hip.h")])
 
 
 def source_digest() -> str:
-    """sha256 (16 hex digits) over every kernel source, header and table of the library plus the compile flags: what a measurement taken on
+    """sha256 (16 hex digits) over every source, header and table of the library's frame, field and stand-alone kernels plus the compile flags: what a measurement taken on
     one tree stamps itself with (tools/pmc_summary.py) and what bench.py compares a committed PMC summary against (`traffic_stale`).
     Content, not mtimes: a snapshot on the GPU box or a fresh checkout has new mtimes and the same digest."""
     import hashlib
@@ -58,7 +74,12 @@ def source_digest() -> str:
 
 def _compile(src, force, extra=(), obj_dir=OBJ_DIR, drop=()):
     obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
-    newest = max(os.path.getmtime(p) for p in [src, __file__, *headers()])
+    train = os.path.dirname(src) == TRAIN_DIR
+    if train:
+        obj_dir = os.path.join(obj_dir, "train")
+        obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
+        extra = (*extra, *TRAIN_FLAGS)
+    newest = max(os.path.getmtime(p) for p in [src, __file__, *(train_headers() if train else headers())])
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= newest:
         return obj, False
     cmd = [HIPCC, *[f for f in COMMON if f not in drop], *PER_FILE.get(os.path.basename(src), ()), *extra, "-x", "hip", "-c", src, "-o", obj, "-I", HERE,
@@ -66,8 +87,9 @@ def _compile(src, force, extra=(), obj_dir=OBJ_DIR, drop=()):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-    if r.stderr.strip():
-        sys.stderr.write(r.stderr)
+    said = "".join(line for line in r.stderr.splitlines(True) if "packed-fp32-ops" not in line)      # the host pass does not know the feature
+    if said.strip():
+        sys.stderr.write(said)
     return obj, True
 
 
@@ -82,9 +104,9 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, varia
     obj_dir = OBJ_DIR + (f"_{tag}" if tag else "")
     out = OUT.replace(".so", f"_{tag}.so") if tag else OUT
     extra = (("-DGF_TRACE",) if trace else ()) + tuple(defines)
-    os.makedirs(obj_dir, exist_ok=True)
+    os.makedirs(os.path.join(obj_dir, "train"), exist_ok=True)
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-        results = list(ex.map(lambda s: _compile(s, force, extra, obj_dir, tuple(drop_flags)), sources()))
+        results = list(ex.map(lambda s: _compile(s, force, extra, obj_dir, tuple(drop_flags)), [*sources(), *train_sources()]))
     objs = [o for o, _ in results]
     if force or any(ch for _, ch in results) or not os.path.exists(out):
         cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *objs, "-o", out, "-lz", "-lpthread"]   # zlib: the PNG frame writer (png_writer.cpp)

@@ -1,0 +1,390 @@
+// AdamW over many tensors in one launch (gf_adamw_step) and the global norm of their gradients (gf_grad_norm); declared in
+// include/geneface_train_hip.h.
+//
+// Both read and write each value once and do some twenty operations on it, so memory bounds them.  The tensors' addresses travel in the kernel
+// arguments (no table in memory that a replayed graph could find changed): a launch takes as many tensors as 4 KB of arguments hold, and every
+// workgroup finds its tensor by one comparison per lane with the first workgroups of all of them.
+#include "../common.hpp"
+#include "elem.hpp"
+#include "geneface_train_hip.h"
+
+namespace gf {
+
+constexpr int kThreads = 256;
+constexpr int kTensors = 56;              // per launch: 56 x 64 bytes + first workgroups + scalars < 4096
+constexpr uint64_t kNarrow = 1ull << 63;  // flag in n: an address of this tensor is no multiple of four values
+
+struct AdamwArgs {
+    gf_adamw_tensor_t t[kTensors];
+    uint32_t first[kTensors];             // first workgroup of each tensor, 0xffffffff behind the last
+    double beta1, beta2, lr;
+    float eps, weight_decay, max_norm;
+    uint32_t chunk;                       // values per workgroup, a multiple of 1024
+    const float* lr_device;
+    const float* grad_scale;
+    const float* found_inf;
+    const float* grad_norm;
+    uint32_t count;
+    uint32_t count_steps;                 // 1: every tensor has one workgroup, which counts its step itself
+};
+static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
+
+struct Hyper { float shrink, om_beta1, beta2, om_beta2, rate, inv_root, eps, grad; };
+
+__device__ __forceinline__ double pow_int(double b, uint32_t t) {
+    double r = 1.0;
+    for (; t; t >>= 1, b *= b) if (t & 1) r *= b;
+    return r;
+}
+
+// Scalars of one tensor in 64 bits, rounded once.  1 - beta^t keeps its digits at small t that way.
+__device__ __forceinline__ Hyper hyper_of(const AdamwArgs& a, float t) {
+    const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
+    const uint32_t ti = (uint32_t)t;
+    Hyper h;
+    h.shrink = (float)(1.0 - lr * (double)a.weight_decay);
+    h.om_beta1 = (float)(1.0 - a.beta1);
+    h.beta2 = (float)a.beta2;
+    h.om_beta2 = (float)(1.0 - a.beta2);
+    h.rate = (float)(lr / (1.0 - pow_int(a.beta1, ti)));
+    h.inv_root = (float)(1.0 / sqrt(1.0 - pow_int(a.beta2, ti)));
+    h.eps = a.eps;
+    double c = a.grad_scale ? 1.0 / (double)*a.grad_scale : 1.0;
+    if (a.grad_norm) {
+        const double q = (double)a.max_norm / ((double)*a.grad_norm + 1e-6);
+        c *= q >= 1.0 ? 1.0 : q;          // a norm that is no number leaves none
+    }
+    h.grad = (float)c;
+    return h;
+}
+
+__device__ __forceinline__ float moment1(const Hyper& h, float m, float g) { return m + h.om_beta1 * (g - m); }
+__device__ __forceinline__ float moment2(const Hyper& h, float v, float g) { return h.beta2 * v + h.om_beta2 * g * g; }
+__device__ __forceinline__ float updated(const Hyper& h, float p, float m, float r) { return p * h.shrink - h.rate * m / (r * h.inv_root + h.eps); }
+
+__device__ __forceinline__ uint32_t tensor_of(const AdamwArgs& a, uint32_t block) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t has = __ballot(lane < kTensors && a.first[lane < kTensors ? lane : 0] <= block);
+    return __builtin_amdgcn_readfirstlane((uint32_t)__popcll(has) - 1u);
+}
+
+// 32-bit moments: four consecutive values a thread.
+template <typename T>
+__device__ __forceinline__ void step32(const gf_adamw_tensor_t& t, const Hyper& h, uint64_t begin, uint64_t end, bool wide) {
+    T* p = (T*)t.p;
+    const T* g = (const T*)t.g;
+    float *m = (float*)t.m, *v = (float*)t.v;
+    for (uint64_t i = begin + threadIdx.x * 4; i < end; i += kThreads * 4) {
+        const int left = (int)min((uint64_t)4, end - i);
+        float fp[4], fg[4], fm[4], fv[4];
+        load4_of(g + i, left, wide, fg);
+        load4_of(m + i, left, wide, fm);
+        load4_of(v + i, left, wide, fv);
+        load4_of(p + i, left, wide, fp);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float x = fg[k] * h.grad;
+            fm[k] = moment1(h, fm[k], x);
+            fv[k] = moment2(h, fv[k], x);
+            fp[k] = updated(h, fp[k], fm[k], sqrtf(fv[k]));
+        }
+        store4_of(m + i, left, wide, fm);
+        store4_of(v + i, left, wide, fv);
+        store4_of(p + i, left, wide, fp);
+    }
+}
+
+// ---- 8-bit moments -------------------------------------------------------------------------------------------------------------------------
+// A block of 128 values has one 32-bit scale a / 448, a its largest magnitude (2^-100 at least, so that 448 / a is finite).  Sixteen lanes share a
+// block: lane j holds values 4j .. 4j+3 and 64+4j .. 64+4j+3, so that every load of a row of lanes is 256 consecutive bytes of 32-bit values.
+// Rounding to nearest would lose every change below half a spacing (up to 6 % of the value; the second moment moves by 1 - beta2 a step).  The
+// value is therefore rounded to floor(value / spacing + u) with u the fractional part of index phi_1 + step phi_2 (a two-dimensional Weyl
+// sequence): over successive steps u is evenly spread, so the stored values are right on average, with no random numbers and no state.
+constexpr uint32_t kDitherIndex = 3242174889u, kDitherStep = 2447445414u;     // 2^32 / rho, 2^32 / rho^2; rho the real root of x^3 = x + 1
+constexpr float kTiny = 7.888609052210118e-31f;                                // 2^-100
+
+// |y| <= 448 to its e4m3 code without the sign.  u20: the dither, 20 bits: as many as a 32-bit value has below the three that e4m3 keeps.
+__device__ __forceinline__ uint32_t encode_e4m3(float y, uint32_t u20) {
+    const uint32_t b = __float_as_uint(y);
+    const uint32_t normal = min(((b + u20) >> 20) - (120u << 3), 0x7eu);
+    const uint32_t small = (uint32_t)(y * 512.0f + (float)u20 * 0x1p-20f);     // below 2^-6 the spacing is 2^-9
+    const uint32_t code = b < 0x3c800000u ? small : normal;
+    return b > 0x7f800000u ? 0x7fu : code;                                     // not a number
+}
+
+__device__ __forceinline__ void decode4(uint32_t w, float scale, float out[4]) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    out[0] = lo[0] * scale; out[1] = lo[1] * scale; out[2] = hi[0] * scale; out[3] = hi[1] * scale;
+}
+
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int left, bool wide) {
+    if (wide && left >= 4) return *reinterpret_cast<const uint32_t*>(src);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < left) w |= (uint32_t)src[i] << (8 * i);
+    return w;
+}
+__device__ __forceinline__ void store_codes(uint8_t* dst, uint32_t w, int left, bool wide) {
+    if (wide && left >= 4) { *reinterpret_cast<uint32_t*>(dst) = w; return; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < left) dst[i] = (uint8_t)(w >> (8 * i));
+}
+
+template <typename T>
+__device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h, uint64_t begin, uint64_t end, bool wide, uint32_t word) {
+    T* p = (T*)t.p;
+    const T* g = (const T*)t.g;
+    uint8_t *m = (uint8_t*)t.m, *v = (uint8_t*)t.v;
+    const int lane16 = threadIdx.x & 15;
+    // all lanes of a row run the same blocks; a ragged last block is whole lanes with nothing left
+    for (uint64_t b = begin / 128 + (threadIdx.x >> 4); b * 128 < end; b += kThreads / 16) {
+        const uint64_t i0 = b * 128 + 4 * lane16;
+        float fp[8], fg[8], fm[8], fr[8];
+        int left[2];
+        const float ms = t.m_scale[b], vs = t.v_scale[b];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const uint64_t i = i0 + 64 * q;
+            left[q] = i < end ? (int)min((uint64_t)4, end - i) : 0;
+            const uint64_t at = left[q] ? i : begin;
+            load4_of(g + at, left[q], wide, fg + 4 * q);
+            load4_of(p + at, left[q], wide, fp + 4 * q);
+            decode4(load_codes(m + at, left[q], wide), ms, fm + 4 * q);
+            decode4(load_codes(v + at, left[q], wide), vs, fr + 4 * q);
+        }
+        uint32_t am = 0, ar = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float x = fg[k] * h.grad;
+            fm[k] = moment1(h, fm[k], x);
+            fr[k] = sqrtf(moment2(h, fr[k] * fr[k], x));
+            fp[k] = updated(h, fp[k], fm[k], fr[k]);
+            const bool there = (k & 3) < left[k >> 2];
+            am = max(am, there ? abs_bits(fm[k]) : 0u);
+            ar = max(ar, there ? abs_bits(fr[k]) : 0u);
+        }
+        // as integers: what is no number stays the largest and makes the whole block none
+        const uint32_t bm = row_max_u32(am), br = row_max_u32(ar);
+        const float a_m = bm > 0x7f800000u ? __uint_as_float(bm) : fmaxf(__uint_as_float(bm), kTiny);
+        const float a_r = br > 0x7f800000u ? __uint_as_float(br) : fmaxf(__uint_as_float(br), kTiny);
+        const float inv_m = 448.0f / a_m, inv_r = 448.0f / a_r;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            uint32_t wm = 0, wr = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t u = ((uint32_t)(i0 + 64 * q + k) * kDitherIndex + word) >> 12;
+                const float fm_ = fm[4 * q + k], fr_ = fr[4 * q + k];
+                const uint32_t cm = encode_e4m3(fabsf(fm_ * inv_m), u) | ((__float_as_uint(fm_) >> 24) & 0x80u);
+                uint32_t cr = encode_e4m3(fr_ * inv_r, u ^ 0x80000u);
+                cr = (cr == 0 && fr_ > 0.0f) ? 1u : cr;      // a second moment above zero stays so: m / sqrt(v) must not meet a lost one
+                wm |= cm << (8 * k);
+                wr |= cr << (8 * k);
+            }
+            if (left[q]) {
+                const uint64_t i = i0 + 64 * q;
+                store_codes(m + i, wm, left[q], wide);
+                store_codes(v + i, wr, left[q], wide);
+                store4_of(p + i, left[q], wide, fp + 4 * q);
+            }
+        }
+        if (lane16 == 0) { t.m_scale[b] = a_m / 448.0f; t.v_scale[b] = a_r / 448.0f; }
+    }
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(kThreads) void k_adamw(const AdamwArgs a) {
+    if (a.found_inf && *a.found_inf != 0.0f) return;
+    const uint32_t at = tensor_of(a, blockIdx.x);
+    const gf_adamw_tensor_t t = a.t[at];
+    const uint64_t n = t.n & ~kNarrow, begin = (uint64_t)(blockIdx.x - a.first[at]) * a.chunk;
+    const bool wide = !(t.n & kNarrow);
+    const float now = *t.step + 1.0f;
+    const Hyper h = hyper_of(a, now);
+    const uint64_t end = min(n, begin + a.chunk);
+    if constexpr (BITS == 32) step32<T>(t, h, begin, end, wide);
+    else step8<T>(t, h, begin, end, wide, (uint32_t)now * kDitherStep);
+    if (a.count_steps) {
+        __syncthreads();                  // the tensor's only workgroup: every thread has read the count
+        if (threadIdx.x == 0) *t.step = now;
+    }
+}
+
+// The counts of tensors with several workgroups: raised when all of those have read them, i.e. by the next launch of the stream.
+__global__ void k_count_steps(const AdamwArgs a) {
+    if (a.found_inf && *a.found_inf != 0.0f) return;
+    if (threadIdx.x < a.count) *a.t[threadIdx.x].step += 1.0f;
+}
+
+template <typename T>
+static void launch_adamw(const AdamwArgs& a, uint32_t blocks, uint32_t bits, hipStream_t s) {
+    if (bits == 32) k_adamw<T, 32><<<blocks, kThreads, 0, s>>>(a);
+    else k_adamw<T, 8><<<blocks, kThreads, 0, s>>>(a);
+}
+
+// ---- the gradients' norm -------------------------------------------------------------------------------------------------------------------
+constexpr int kNormTensors = 140;         // per launch, as many as 4 KB of arguments hold
+constexpr uint32_t kNormBlocks = 2048;    // sums of one call, apart from one per tensor
+
+struct NormArgs {
+    gf_norm_tensor_t t[kNormTensors];
+    uint32_t first[kNormTensors];
+    uint64_t chunk;                       // values per workgroup, a multiple of 4096
+    double* sums;
+};
+static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
+
+__device__ __forceinline__ double block_sum(double x, double* lds) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    double r = 0;
+    for (uint32_t w = 0; w < blockDim.x / 64; ++w) r += lds[w];
+    return r;
+}
+
+// Squares are added up in 64 bits: a 32-bit square leaves the type's range at 1e19 and at 1e-23, and the sum is one over all values of a model.
+template <typename T>
+__device__ __forceinline__ double squares(const T* g, uint64_t begin, uint64_t end, bool wide) {
+    double s[4] = {0, 0, 0, 0};
+    for (uint64_t i = begin + threadIdx.x * 4; i < end; i += kThreads * 16) {
+        float f[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint64_t j = i + q * kThreads * 4;
+            const int left = j < end ? (int)min((uint64_t)4, end - j) : 0;
+            load4_of(g + (left ? j : begin), left, wide, f[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] = fma((double)f[q][k], (double)f[q][k], s[k]);
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+__global__ __launch_bounds__(kThreads) void k_norm(const NormArgs a) {
+    __shared__ double lds[kThreads / 64];
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t at = 0;
+    for (uint32_t r = 0; r < kNormTensors; r += 64)
+        at += (uint32_t)__popcll(__ballot(r + lane < kNormTensors && a.first[r + lane < kNormTensors ? r + lane : 0] <= blockIdx.x));
+    at = __builtin_amdgcn_readfirstlane(at) - 1;
+    const gf_norm_tensor_t t = a.t[at];
+    const uint64_t n = t.n & ~kNarrow, begin = (blockIdx.x - a.first[at]) * a.chunk, end = min(n, begin + a.chunk);
+    const bool wide = !(t.n & kNarrow);
+    double s;
+    if (t.dtype == F32) s = squares((const float*)t.g, begin, end, wide);
+    else if (t.dtype == BF16) s = squares((const __bf16*)t.g, begin, end, wide);
+    else s = squares((const _Float16*)t.g, begin, end, wide);
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(1024) void k_norm_finish(const double* sums, uint32_t count, const float* grad_scale, float* out) {
+    __shared__ double lds[16];
+    double s = 0;
+    for (uint32_t i = threadIdx.x; i < count; i += 1024) s += sums[i];
+    s = block_sum(s, lds);
+    if (threadIdx.x == 0) *out = (float)(sqrt(s) / (grad_scale ? (double)*grad_scale : 1.0));
+}
+
+static uint32_t elem_bytes(uint32_t dtype) { return dtype == F32 ? 4 : 2; }
+static bool off(const void* p, uint32_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
+
+}  // namespace gf
+
+using namespace gf;
+
+GF_EXPORT int gf_adamw_step(const gf_adamw_t* d, void* stream) {
+    if (!d) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: null descriptor");
+    if (d->count == 0) return GF_OK;
+    if (!d->tensors_host) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: null tensor list");
+    if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: unknown dtype %u", d->dtype);
+    if (d->state_bits != 32 && d->state_bits != 8) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: state_bits must be 32 or 8, got %u", d->state_bits);
+    if (!(d->beta1 >= 0 && d->beta1 < 1 && d->beta2 >= 0 && d->beta2 < 1)) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: betas must be in [0, 1)");
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < d->count; ++i) {
+        const gf_adamw_tensor_t& t = d->tensors_host[i];
+        if (!t.step || (t.n && (!t.p || !t.g || !t.m || !t.v || (d->state_bits == 8 && (!t.m_scale || !t.v_scale)))))
+            return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: null pointer in tensor %u", i);
+        if (t.n >> 40) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: tensor %u has too many values", i);
+        total += t.n;
+    }
+    // Values per workgroup: as many workgroups as keep the chip's 256 CUs busy where there is work for them, few enough that each amortises its
+    // scalars (two powers in 64 bits, about half a microsecond) where there is more.
+    uint32_t chunk = 1024;
+    while (chunk < 8192 && total / chunk > 4096) chunk *= 2;
+    while (total / chunk > (1ull << 30)) chunk *= 2;
+
+    AdamwArgs a;
+    a.beta1 = d->beta1; a.beta2 = d->beta2; a.lr = d->lr;
+    a.eps = (float)d->eps; a.weight_decay = (float)d->weight_decay; a.max_norm = (float)d->max_norm;
+    a.chunk = chunk;
+    a.lr_device = d->lr_device; a.grad_scale = d->grad_scale; a.found_inf = d->found_inf; a.grad_norm = d->grad_norm;
+    const uint32_t eb = elem_bytes(d->dtype), sb = d->state_bits / 8;
+    for (uint32_t i = 0; i < d->count;) {
+        uint32_t k = 0, blocks = 0;
+        bool several = false;
+        for (; i < d->count && k < kTensors; ++i, ++k) {
+            gf_adamw_tensor_t t = d->tensors_host[i];
+            const uint32_t need = t.n ? (uint32_t)((t.n + chunk - 1) / chunk) : 1;       // an empty tensor's step is counted too
+            several |= need > 1;
+            if (off(t.p, 4 * eb) || off(t.g, 4 * eb) || off(t.m, 4 * sb) || off(t.v, 4 * sb)) t.n |= kNarrow;
+            a.t[k] = t;
+            a.first[k] = blocks;
+            blocks += need;
+        }
+        a.count = k;
+        a.count_steps = !several;
+        for (; k < kTensors; ++k) { a.t[k] = a.t[0]; a.first[k] = 0xffffffffu; }
+        const hipStream_t s = gf_stream(stream);
+        if (d->dtype == F32) launch_adamw<float>(a, blocks, d->state_bits, s);
+        else if (d->dtype == BF16) launch_adamw<__bf16>(a, blocks, d->state_bits, s);
+        else launch_adamw<_Float16>(a, blocks, d->state_bits, s);
+        if (several) k_count_steps<<<1, 64, 0, s>>>(a);
+        if (const int rc = gf_check_launch("gf_adamw_step")) return rc;
+    }
+    return GF_OK;
+}
+
+GF_EXPORT uint64_t gf_grad_norm_workspace_bytes(uint32_t count) { return 8ull * ((uint64_t)kNormBlocks + count); }
+
+GF_EXPORT int gf_grad_norm(const gf_grad_norm_t* d, void* stream) {
+    if (!d) return gf_set_error(GF_ERR_INVALID, "gf_grad_norm: null descriptor");
+    if (!d->norm_out || !d->workspace || (d->count && !d->tensors_host)) return gf_set_error(GF_ERR_INVALID, "gf_grad_norm: null pointer");
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < d->count; ++i) {
+        const gf_norm_tensor_t& t = d->tensors_host[i];
+        if (t.n && !t.g) return gf_set_error(GF_ERR_INVALID, "gf_grad_norm: null pointer in tensor %u", i);
+        if (t.dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_grad_norm: unknown dtype %u in tensor %u", t.dtype, i);
+        if (t.n >> 40) return gf_set_error(GF_ERR_INVALID, "gf_grad_norm: tensor %u has too many values", i);
+        total += t.n;
+    }
+    const hipStream_t s = gf_stream(stream);
+    NormArgs a;
+    a.chunk = (total / kNormBlocks + 4096) / 4096 * 4096;
+    uint32_t done = 0;
+    for (uint32_t i = 0; i < d->count;) {
+        int k = 0;
+        uint32_t blocks = 0;
+        for (; i < d->count && k < kNormTensors; ++i) {
+            gf_norm_tensor_t t = d->tensors_host[i];
+            if (!t.n) continue;
+            const uint32_t need = (uint32_t)((t.n + a.chunk - 1) / a.chunk);
+            if (off(t.g, 4 * elem_bytes(t.dtype))) t.n |= kNarrow;
+            a.t[k] = t;
+            a.first[k++] = blocks;
+            blocks += need;
+        }
+        if (!blocks) break;
+        for (; k < kNormTensors; ++k) { a.t[k] = a.t[0]; a.first[k] = 0xffffffffu; }
+        a.sums = (double*)d->workspace + done;
+        k_norm<<<blocks, kThreads, 0, s>>>(a);
+        done += blocks;
+    }
+    k_norm_finish<<<1, 1024, 0, s>>>((const double*)d->workspace, done, d->grad_scale, d->norm_out);
+    return gf_check_launch("gf_grad_norm");
+}

@@ -1,4 +1,4 @@
-"""ctypes binding of libgeneface_hip.so (C ABI: include/geneface_hip.h).
+"""ctypes binding of libgeneface_hip.so (C ABI: include/geneface_hip.h and include/geneface_train_hip.h).
 
 There is NO fallback: if the shared library cannot be loaded, or a call reports an error, a
 RuntimeError is raised.  Nothing here (or anywhere under geneface_amd/) imports the CPU oracle.
@@ -14,6 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # GF_HIP_LIB selects another build of the same library (tools/trace_head.py points it at the instrumented one)
 LIB_PATH = os.environ.get("GF_HIP_LIB") or os.path.join(_HERE, "csrc", "libgeneface_hip.so")
 HEADER_PATH = os.path.join(_HERE, "..", "include", "geneface_hip.h")
+TRAIN_HEADER_PATH = os.path.join(_HERE, "..", "include", "geneface_train_hip.h")
 
 _lock = threading.Lock()
 _lib = None
@@ -48,7 +49,7 @@ def header_prototypes(path: str = HEADER_PATH):
 
 
 def _bind(lib):
-    for ret, name, args in header_prototypes():
+    for ret, name, args in header_prototypes() + header_prototypes(TRAIN_HEADER_PATH):
         fn = getattr(lib, name)  # AttributeError here == header/library mismatch: fail loudly
         fn.restype = {"int": C.c_int, "uint32_t": C.c_uint32, "uint64_t": C.c_uint64, "void*": C.c_void_p}.get(ret, C.c_char_p)
         argtypes = []

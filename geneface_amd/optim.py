@@ -1,0 +1,279 @@
+"""AdamW over many tensors in one launch, with moments in 32 or 8 bits, and the global norm of their gradients.
+
+What the reference's tasks build around the model (tasks/radnerfs/radnerf.py:53-72: Adam over the networks and the grid tables, eps 1e-15) as
+kernels of this library: `AdamW` is a torch optimizer (param groups, state dict, GradScaler), `adamw_step` and `grad_norm` are the two calls below
+it.  With `weight_decay=0` it is Adam.
+
+8-bit moments: e4m3 codes with one 32-bit scale for each 128 consecutive values of a tensor, max(largest magnitude, 2^-100) / 448.  The second
+moment is held as its square root, which halves the range it needs.  Codes are rounded by a dither that depends on the step and on the value's
+index only, so a step is reproducible and changes far below the format's spacing add up over the steps; a second moment above zero never becomes
+zero.  A block that meets a gradient that is no finite number is none afterwards (all 128 values).
+
+Everything is done on the current stream of the tensors' device and may be captured into a graph; a graph keeps the addresses, and numbers given
+as Python numbers (`lr` as a one-element tensor on the device stays adjustable).
+"""
+import ctypes as C
+import math
+
+import torch
+
+from .lib import check, current_stream, lib
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+BLOCK = 128
+
+_vp = C.c_void_p
+
+
+class GfAdamw(C.Structure):
+    """ctypes mirror of gf_adamw_t (include/geneface_train_hip.h)."""
+    _fields_ = [("tensors_host", _vp), ("count", C.c_uint32), ("dtype", C.c_uint32), ("state_bits", C.c_uint32), ("_pad", C.c_uint32)] + \
+               [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + \
+               [(n, _vp) for n in ("lr_device", "grad_scale", "found_inf", "grad_norm")]
+
+
+class GfGradNorm(C.Structure):
+    """ctypes mirror of gf_grad_norm_t."""
+    _fields_ = [("tensors_host", _vp), ("count", C.c_uint32), ("_pad", C.c_uint32)] + [(n, _vp) for n in ("grad_scale", "norm_out", "workspace")]
+
+
+# a step asks these of hundreds of tensors: mapped over whole lists they cost a tenth of a microsecond each
+_ptr, _numel, _contiguous, _device_index = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype, _layout = torch.Tensor.dtype.__get__, torch.Tensor.layout.__get__
+
+
+def _same_device(name, tensors, device):
+    if device.type != "cuda":
+        raise RuntimeError(f"{name} must be CUDA tensors")
+    if {*map(_device_index, tensors)} != {device.index}:
+        raise RuntimeError(f"{name} must all be on {device}")
+
+
+def _scalar(name, t, device):
+    """Address of one float32 on the device, or None."""
+    if t is None:
+        return None
+    if not torch.is_tensor(t) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        raise RuntimeError(f"{name} must be one float32 value on {device}")
+    return t.data_ptr()
+
+
+def grad_norm(grads, grad_scale=None):
+    """sqrt(sum of the squares of all `grads`) / grad_scale as a float32 tensor without dimensions, added up in 64 bits in a fixed order.
+
+    grads: tensors of float32, bfloat16 or float16 on one device (None entries are left out).  grad_scale: one float32 on that device, the
+    factor the gradients carry (GradScaler's scale).  Infinities and NaN among the gradients give an infinite norm or NaN."""
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        raise RuntimeError("grad_norm: no gradients")
+    if {*map(_layout, grads)} != {torch.strided}:
+        raise RuntimeError("grad_norm: sparse gradients are not supported")
+    dev = grads[0].device
+    dtypes = [DTYPES.get(d) for d in map(_dtype, grads)]
+    if None in dtypes:
+        raise RuntimeError("grad_norm: gradients must be float32, bfloat16 or float16")
+    _same_device("grad_norm: the gradients", grads, dev)
+    with torch.cuda.device(dev):
+        if not all(map(_contiguous, grads)):
+            grads = [g.contiguous() for g in grads]
+        scale = _scalar("grad_scale", grad_scale, dev)
+        L, n = lib(), len(grads)
+        out = torch.empty((), dtype=torch.float32, device=dev)
+        workspace = torch.empty(L.gf_grad_norm_workspace_bytes(n) // 8, dtype=torch.float64, device=dev)
+        table = (C.c_uint64 * (3 * n))()
+        table[0::3], table[1::3], table[2::3] = list(map(_ptr, grads)), list(map(_numel, grads)), dtypes
+        d = GfGradNorm(C.addressof(table), n, 0, scale, out.data_ptr(), workspace.data_ptr())
+        check(L.gf_grad_norm(C.byref(d), current_stream(dev)))
+    return out
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, exp_avg_scales=None,
+               exp_avg_sq_scales=None, grad_scale=None, found_inf=None, grad_norm=None, max_norm=None):
+    """One AdamW step over lists of tensors, in place, in one launch for every 56 tensors of a type.
+
+    params, grads: float32, bfloat16 or float16, gradients of their parameter's type and size.  exp_avgs, exp_avg_sqs: float32 of the same sizes,
+    or -- with exp_avg_scales and exp_avg_sq_scales, lists of float32 [ceil(numel / 128)] -- float8_e4m3fn.  steps: one float32 each, the number of
+    steps taken so far.  Everything on one device; all but gradients must be contiguous.
+
+    lr: a number, or one float32 on the device.  grad_scale: the factor that the gradients carry.  found_inf: where it is not 0 nothing is
+    changed, the step counts included.  grad_norm, max_norm: gradients are multiplied by min(1, max_norm / (grad_norm + 1e-6)); both or neither.
+    grad_scale, found_inf, grad_norm: one float32 on the device each.  Gradients are only read: they keep their factor."""
+    eight = exp_avg_scales is not None or exp_avg_sq_scales is not None
+    lists = [params, grads, exp_avgs, exp_avg_sqs, steps] + ([exp_avg_scales, exp_avg_sq_scales] if eight else [])
+    if any(v is None for v in lists):
+        raise RuntimeError("adamw_step: exp_avg_scales and exp_avg_sq_scales must both be given for 8-bit moments")
+    lists = [list(v) for v in lists]
+    params, grads, exp_avgs, exp_avg_sqs, steps = lists[:5]
+    n = len(params)
+    if any(len(v) != n for v in lists):
+        raise RuntimeError(f"adamw_step: lists of unlike lengths {[len(v) for v in lists]}")
+    beta1, beta2 = map(float, betas)
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
+        raise ValueError(f"adamw_step: betas must be in [0, 1), got {betas}")
+    if (grad_norm is None) != (max_norm is None):
+        raise RuntimeError("adamw_step: grad_norm and max_norm go together")
+    if not n:
+        return
+    dev = params[0].device
+    sizes = list(map(_numel, params))
+    if {*map(_layout, grads)} != {torch.strided}:
+        raise RuntimeError("adamw_step: sparse gradients are not supported")
+    types = list(map(_dtype, params))
+    if list(map(_dtype, grads)) != types:
+        raise RuntimeError("adamw_step: a gradient must have its parameter's dtype")
+    kinds = set(types)
+    if not kinds <= DTYPES.keys():
+        raise RuntimeError("adamw_step: parameters must be float32, bfloat16 or float16")
+    if any(list(map(_numel, v)) != sizes for v in lists[1:4]):
+        raise RuntimeError("adamw_step: gradients and moments must have their parameter's size")
+    state = torch.float8_e4m3fn if eight else torch.float32
+    if {*map(_dtype, exp_avgs), *map(_dtype, exp_avg_sqs)} != {state}:
+        raise RuntimeError(f"adamw_step: moments must be {state} {'with' if eight else 'without'} scales")
+    if {*map(_dtype, steps)} != {torch.float32} or {*map(_numel, steps)} != {1}:
+        raise RuntimeError("adamw_step: each step must be one float32 value")
+    if eight:
+        blocks = [-(-k // BLOCK) for k in sizes]
+        for v in lists[5:]:
+            if {*map(_dtype, v)} != {torch.float32} or list(map(_numel, v)) != blocks:
+                raise RuntimeError("adamw_step: scales must be float32 with one value for each 128 of the parameter")
+    _same_device("adamw_step: all tensors", [t for v in lists for t in v], dev)
+    if not all(map(_contiguous, grads)):
+        with torch.cuda.device(dev):
+            grads = lists[1] = [g.contiguous() for g in grads]
+    if not all(map(_contiguous, [t for v in lists for t in v])):
+        raise RuntimeError("adamw_step: parameters and their state must be contiguous tensors")
+    pointers = [list(map(_ptr, v)) for v in lists]
+    for k, v in enumerate(pointers):
+        if k != 1 and len({*v}) != n and (k == 4 or len({a for a, size in zip(v, sizes) if size}) != n - sizes.count(0)):      # (empty tensors have no address)
+            raise RuntimeError("adamw_step: the same tensor is given twice")
+    lr_device = None
+    if torch.is_tensor(lr):
+        if lr.is_cuda:
+            lr, lr_device = 0.0, _scalar("lr", lr, dev)
+        else:
+            lr = float(lr)
+    scalars = [_scalar(k, t, dev) for k, t in (("grad_scale", grad_scale), ("found_inf", found_inf), ("grad_norm", grad_norm))]
+    L = lib()
+    with torch.cuda.device(dev):
+        for kind in sorted(kinds, key=DTYPES.get):
+            pick = pointers + [sizes]
+            if len(kinds) > 1:
+                at = [i for i in range(n) if types[i] == kind]
+                pick = [[v[i] for i in at] for v in pick]
+            p, g, m, v, step = pick[:5]
+            count = len(p)
+            table = (C.c_uint64 * (8 * count))()
+            table[0::8], table[1::8], table[2::8], table[3::8], table[6::8], table[7::8] = p, g, m, v, step, pick[-1]
+            if eight:
+                table[4::8], table[5::8] = pick[5], pick[6]
+            d = GfAdamw(C.addressof(table), count, DTYPES[kind], 8 if eight else 32, 0, float(lr), beta1, beta2, float(eps), float(weight_decay),
+                        math.inf if max_norm is None else float(max_norm), lr_device, *scalars)
+            check(L.gf_adamw_step(C.byref(d), current_stream(dev)))
+    torch.autograd.graph.increment_version([t for k, v in enumerate(lists) if k != 1 for t in v])      # written through raw pointers
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update (without amsgrad and maximize) in one launch for all tensors of a param group and type.
+
+    state_bits: 32, or 8 for moments of one byte each and a scale per 128 values (16 bytes moved per float32 parameter instead of 28).
+    max_grad_norm: clips the gradients of ALL groups to this norm inside the step; the norm of the last step stays in `last_grad_norm`.  The
+    gradients themselves are not changed.  Under torch.amp.GradScaler unscaling and the skipped step after an overflow happen inside the kernel, without a
+    host sync.  lr may be a one-element float32 tensor on the device, so that a captured step follows a schedule."""
+
+    _step_supports_amp_scaling = True      # GradScaler.step hands its scale and found_inf over as attributes and calls step() itself
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=32, max_grad_norm=None):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if not torch.is_tensor(lr) and not lr >= 0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError(f"Invalid betas: {betas}")
+        if not eps >= 0:
+            raise ValueError(f"Invalid epsilon value: {eps}")
+        if not weight_decay >= 0:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
+        self.state_bits, self.max_grad_norm, self.last_grad_norm = state_bits, max_grad_norm, None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _keys(self):
+        return ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if self.state_bits == 8 else ())
+
+    def _init_state(self, p):
+        state = self.state[p]
+        if not state:
+            if p.dtype not in DTYPES or not p.is_cuda or not p.is_contiguous():
+                raise RuntimeError("AdamW: parameters must be contiguous CUDA tensors of float32, bfloat16 or float16")
+            state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            for k in self._keys():
+                if k.endswith("scale"):
+                    state[k] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
+                elif self.state_bits == 8:
+                    state[k] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+                else:
+                    state[k] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups = [[p for p in g["params"] if p.grad is not None] for g in self.param_groups]
+        used = [p for g in groups for p in g]
+        if not used:
+            return loss
+        devices = {p.device for p in used}
+        scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        norm = None
+        if self.max_grad_norm is not None:
+            if len(devices) > 1:
+                raise RuntimeError("AdamW: max_grad_norm needs all parameters on one device")
+            norm = grad_norm([p.grad for p in used], grad_scale=None if scale is None else scale.to(used[0].device))
+            self.last_grad_norm = norm
+        for group, params in zip(self.param_groups, groups):
+            for dev in sorted({p.device for p in params}, key=str):
+                ps = [p for p in params if p.device == dev] if len(devices) > 1 else params
+                states = [self._init_state(p) for p in ps]
+                column = lambda k: [s[k] for s in states]      # noqa: E731
+                there = lambda t: None if t is None else t.to(dev)      # noqa: E731
+                eight = self.state_bits == 8
+                adamw_step(ps, [p.grad for p in ps], column("exp_avg"), column("exp_avg_sq"), column("step"), lr=group["lr"], betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"], exp_avg_scales=column("exp_avg_scale") if eight else None,
+                           exp_avg_sq_scales=column("exp_avg_sq_scale") if eight else None, grad_scale=there(scale), found_inf=there(found),
+                           grad_norm=norm, max_norm=self.max_grad_norm if norm is not None else None)
+        return loss
+
+    def moments(self, p):
+        """(first moment, second moment) of a parameter as new float32 tensors of its shape, whatever they are held in."""
+        s = self.state[p]
+        if self.state_bits == 32:
+            return s["exp_avg"].clone(), s["exp_avg_sq"].clone()
+        wide = lambda k: s[k].float().reshape(-1) * s[k + "_scale"].repeat_interleave(BLOCK)[:p.numel()]      # noqa: E731
+        return wide("exp_avg").view(p.shape), wide("exp_avg_sq").square().view(p.shape)
+
+    def load_state_dict(self, state_dict):
+        """State of this class, or -- with 32-bit moments -- of torch.optim.Adam / AdamW.  Moments keep their own types (torch would cast them to the
+        parameter's)."""
+        want = {k: torch.float8_e4m3fn if self.state_bits == 8 and not k.endswith("scale") else torch.float32 for k in self._keys()}
+        for s in state_dict["state"].values():
+            missing = [k for k in ("step", *want) if k not in s]
+            if missing or any(s[k].dtype != dt for k, dt in want.items()):
+                raise RuntimeError(f"AdamW: the state does not hold {self.state_bits}-bit moments")
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        super().load_state_dict(state_dict)
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            s = state_dict["state"].get(i)
+            if s is None:
+                continue
+            state = {"step": torch.as_tensor(s["step"], dtype=torch.float32).detach().to(p.device, copy=True).reshape(())}
+            for k in want:
+                shape = (-(-p.numel() // BLOCK),) if k.endswith("scale") else p.shape
+                if tuple(s[k].shape) != tuple(shape):
+                    raise RuntimeError(f"AdamW: {k} of shape {tuple(s[k].shape)} for a parameter of shape {tuple(p.shape)}")
+                state[k] = s[k].detach().to(p.device, copy=True).contiguous()
+            self.state[p] = state

@@ -1,0 +1,80 @@
+/*
+ * geneface_train_hip.h -- the part of libgeneface_hip.so's C ABI that a training step needs beside the field's own nodes: AdamW over many
+ * tensors at once, the global norm of their gradients, and block-scaled 8-bit linear products.
+ *
+ * Conventions are those of geneface_hip.h: device pointers unless a name ends in _host, outputs allocated by the caller, `stream` a hipStream_t,
+ * calls only enqueue work, 0 on success and gf_last_error() otherwise.  `dtype` is one of GF_F32 / GF_BF16 / GF_F16.
+ */
+#ifndef GENEFACE_TRAIN_HIP_H
+#define GENEFACE_TRAIN_HIP_H
+
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define GF_F32 0
+#define GF_BF16 1
+#define GF_F16 2
+
+/* One tensor of gf_adamw_step: n values of p (updated), g (read), the moments m and v (updated) and the step count (one float, incremented).
+ * With 32-bit moments m and v are float[n] and the scales NULL.  With 8-bit moments m and v are e4m3 codes [n] and m_scale / v_scale
+ * float[ceil(n / 128)]: m[i] = m_code[i] m_scale[i / 128] and sqrt(v[i]) = v_code[i] v_scale[i / 128]. */
+typedef struct {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    float* step;
+    uint64_t n;
+} gf_adamw_tensor_t;
+
+/* Host descriptor; tensors_host is read during the call.  grad_scale, found_inf, grad_norm and lr_device are one float on the device each, or
+ * NULL.  The gradients that enter are g / grad_scale min(1, max_norm / (grad_norm + 1e-6)).  Where *found_inf is not 0 nothing is changed, the
+ * step counts included.  lr_device replaces lr.  dtype: of p and g.  state_bits: 32 or 8. */
+typedef struct {
+    const gf_adamw_tensor_t* tensors_host;
+    uint32_t count;
+    uint32_t dtype;
+    uint32_t state_bits;
+    uint32_t _pad;
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    const float* lr_device;
+    const float* grad_scale;
+    const float* found_inf;
+    const float* grad_norm;
+} gf_adamw_t;
+
+/* p <- p (1 - lr wd);  m <- m + (1 - beta1)(g - m);  v <- beta2 v + (1 - beta2) g^2;
+ * p <- p - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps), t the incremented step. */
+int gf_adamw_step(const gf_adamw_t* desc, void* stream);
+
+/* One tensor of gf_grad_norm: n values of `dtype`. */
+typedef struct {
+    const void* g;
+    uint64_t n;
+    uint32_t dtype;
+    uint32_t _pad;
+} gf_norm_tensor_t;
+
+/* Host descriptor; tensors_host is read during the call.  norm_out[0] = sqrt(sum over all tensors of g^2) / grad_scale, added up in 64 bits in
+ * a fixed order; grad_scale: one float on the device, or NULL.  workspace: gf_grad_norm_workspace_bytes(count) device bytes of this call's own. */
+typedef struct {
+    const gf_norm_tensor_t* tensors_host;
+    uint32_t count;
+    uint32_t _pad;
+    const float* grad_scale;
+    float* norm_out;
+    void* workspace;
+} gf_grad_norm_t;
+
+uint64_t gf_grad_norm_workspace_bytes(uint32_t count);
+int gf_grad_norm(const gf_grad_norm_t* desc, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -16,6 +16,21 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 
 
+def optimizer_name(args):
+    if args.optimizer != "torch":
+        return "AdamW with 8-bit moments" if args.optimizer == "adamw8" else "library AdamW"
+    return ("foreach" if args.foreach_adam else "fused") + " Adam"
+
+
+def optimizer(args, params):
+    import torch
+    kw = dict(lr=5e-4, betas=(0.9, 0.99), eps=1e-15)
+    if args.optimizer == "torch":
+        return torch.optim.Adam(params, **kw, fused=not args.foreach_adam)
+    from geneface_amd.optim import AdamW
+    return AdamW(params, **kw, weight_decay=0.0, state_bits=8 if args.optimizer == "adamw8" else 32)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--steps", type=int, default=48)
@@ -23,6 +38,8 @@ def main():
     ap.add_argument("--n-rays", type=int, default=65536)
     ap.add_argument("--foreach-adam", action="store_true", help="torch.optim.Adam's default multi-tensor path (what the reference's trainer builds) "
                     "instead of fused=True")
+    ap.add_argument("--optimizer", choices=("torch", "adamw", "adamw8"), default="torch", help="torch.optim.Adam, or geneface_amd.optim.AdamW without weight "
+                    "decay (the same update) with moments in 32 or 8 bits")
     ap.add_argument("--amp", action="store_true", help="fp16 autocast + GradScaler, as the May config trains (lm3d_radnerf.yaml:5 amp: true)")
     ap.add_argument("--amp-f32-field", action="store_true", help="--amp with the exact-fp32 field node under autocast (RADNeRF.amp_field = 'f32': round 5's "
                     "behaviour) instead of the f16 tier")
@@ -78,7 +95,7 @@ def main():
     target = torch.rand(1, 512 * 512, 3, device=dev)
     # fused=True: one multi-tensor kernel, and under a GradScaler the skip-on-overflow decision stays on the device -- the default (foreach)
     # optimizer makes GradScaler.step() read found_inf on the host every step, which serialises host and GPU
-    opt = torch.optim.Adam(model.parameters(), lr=5e-4, betas=(0.9, 0.99), eps=1e-15, fused=not args.foreach_adam)
+    opt = optimizer(args, model.parameters())
     torch.manual_seed(0)
     scaler = torch.amp.GradScaler("cuda", enabled=args.amp)
 
@@ -115,7 +132,7 @@ def main():
     quiet = sorted(h for k, h in enumerate(host) if (args.warmup + k) % hp["update_extra_interval"] != 0)
     print(f"host enqueue per step: median {1e3 * quiet[len(quiet) // 2]:.2f} ms, min {1e3 * quiet[0]:.2f}, max {1e3 * quiet[-1]:.2f} "
           f"(steps without an occupancy refresh); step {1e3 * dt / args.steps:.2f} ms", file=sys.stderr)
-    print(json.dumps({"metric": f"RAD-NeRF head training steps/s (n_rays {args.n_rays}, {('fp16 autocast, field on the ' + ('exact-fp32 node' if args.amp_f32_field else 'f16 tier')) if args.amp else 'fp32'}, {'foreach' if args.foreach_adam else 'fused'} Adam, grid update every 16 steps)", "value": rate,
+    print(json.dumps({"metric": f"RAD-NeRF head training steps/s (n_rays {args.n_rays}, {('fp16 autocast, field on the ' + ('exact-fp32 node' if args.amp_f32_field else 'f16 tier')) if args.amp else 'fp32'}, {optimizer_name(args)}, grid update every 16 steps)", "value": rate,
                       "ms_per_step": 1e3 / rate, "hours_for_250k_steps": 250000 / rate / 3600, "points_last_step": int(model.step_counter[(model.local_step - 1) % 16, 0]),
                       "amp": {"field": getattr(model, "amp_field", "f16"), "backward": getattr(model, "amp_backward", "f16"),
                               "weight_gradients": getattr(model, "amp_wgrad", "fused")} if args.amp else None,
@@ -159,7 +176,7 @@ def main_torso(args):
     for k, p in model.named_parameters():
         if "torso" not in k:
             p.requires_grad_(False)
-    opt = torch.optim.Adam(net, lr=5e-4, betas=(0.9, 0.99), eps=1e-15, fused=not args.foreach_adam)
+    opt = optimizer(args, net)
     opt.add_param_group({"params": emb, "lr": 5e-3, "betas": (0.9, 0.99), "eps": 1e-15})
     torch.manual_seed(0)
     scaler = torch.amp.GradScaler("cuda", enabled=args.amp)
@@ -193,7 +210,7 @@ def main_torso(args):
     dt = time.perf_counter() - t0
     rate = args.steps / dt
     print(json.dumps({"metric": f"RAD-NeRF TORSO training steps/s (head frozen; n_rays {args.n_rays}, {'fp16 autocast' if args.amp else 'fp32'}, "
-                                f"{'foreach' if args.foreach_adam else 'fused'} Adam, torso occupancy update every 16 steps)", "value": rate,
+                                f"{optimizer_name(args)}, torso occupancy update every 16 steps)", "value": rate,
                       "ms_per_step": 1e3 / rate, "hours_for_250k_steps": 250000 / rate / 3600,
                       "masked_pixels_last_step": int((out["torso_alpha_map"] > 0).sum()), "torso_train_dense": bool(model.torso_train_dense), "head_points_last_step": int(model.step_counter[(model.local_step - 1) % 16, 0]),
                       "reference_published": "~4 h for the torso on an RTX 3090 Ti, docs/train_models/train_models.md:93", "data": "synthetic"}))
