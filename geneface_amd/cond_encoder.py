@@ -9,6 +9,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import fp8
+
 _STRIDES = {1: (1, 1, 1, 1), 2: (2, 1, 1, 1), 3: (2, 2, 1, 1), 4: (2, 2, 1, 1), 16: (2, 2, 2, 2)}
 
 
@@ -87,6 +89,10 @@ class _linear_tall(torch.autograd.Function):
 
 
 class MLP(nn.Module):
+    #: "native": torch's products in the layers' type; "fp8": both operands of every product in block-scaled 8 bits, added up in 32 (fp8.py), under
+    #: autograd and without it.  The stand-alone MLP and the op-by-op field (field_impl / render_impl "ops") go by it, the fused kernels do not.
+    precision = "native"
+
     def __init__(self, dim_in, dim_out, dim_hidden, num_layers):
         super().__init__()
         self.dim_in, self.dim_out, self.dim_hidden, self.num_layers = dim_in, dim_out, dim_hidden, num_layers
@@ -95,8 +101,12 @@ class MLP(nn.Module):
             for l in range(num_layers)])
 
     def forward(self, x):
+        if self.precision not in ("native", "fp8"):
+            raise ValueError(f"MLP.precision must be 'native' or 'fp8', got {self.precision!r}")
         for l, layer in enumerate(self.net):
-            if x.dim() == 2 and x.shape[0] >= _TALL and torch.is_grad_enabled() and (x.requires_grad or layer.weight.requires_grad):
+            if self.precision == "fp8":
+                x = fp8.linear(x, layer.weight)
+            elif x.dim() == 2 and x.shape[0] >= _TALL and torch.is_grad_enabled() and (x.requires_grad or layer.weight.requires_grad):
                 x = _linear_tall.apply(x, layer.weight)
             else:
                 x = layer(x)

@@ -1,0 +1,434 @@
+// gf_fp8_matmul and gf_fp8_rows: products of block-scaled 8-bit values on the scaled matrix instructions.
+//
+// A block of 128 has one power-of-two scale, which is what v_mfma_scale_* take (as a byte per lane, for each 32 values): the products of all blocks
+// are added up in the accumulator itself, with no rescaling between them.  Since a block's 128 values share their scale, the order in which
+// they reach a lane does not matter as long as both operands have the same.
+#include "../common.hpp"
+#include "fp8.hpp"
+#include "geneface_train_hip.h"
+
+namespace gf {
+
+struct Operand {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    uint64_t pitch, stride_row, stride_block;      // pitch > 0: scales by row; 0: by tile
+    __device__ __forceinline__ uint64_t step() const { return pitch ? pitch : stride_block; }
+    __device__ __forceinline__ uint64_t at(uint64_t row) const { return pitch ? row : (row >> 7) * stride_row; }
+};
+
+struct MatmulArgs {
+    Operand a, b;
+    uint32_t m, n, blocks, per_split;      // blocks of 128, and how many of them each split adds up
+    uint32_t tiles_m, tiles_n;
+    void* out;                             // [m, n], or with several splits float [splits, m, n]
+};
+
+typedef __attribute__((address_space(3))) void lds_t;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+#define GF_FENCE __builtin_amdgcn_sched_barrier(0)      // the scheduler moves nothing across
+
+// Sixteen codes' products at a time on the bfloat16 matrix instruction, with the blocks' scales multiplied in: exact, since a code has four
+// significant bits and a scale none.
+__device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ float scale_value(int byte) { return __uint_as_float(byte ? (uint32_t)byte << 23 : 0x00400000u); }
+
+// A workgroup of 2 x 2 waves makes a tile of 64 TM x 64 TN of the product, a wave TM x TN tiles of 32 x 32.
+//
+// Blocks of codes come straight from memory to LDS, two of them at a time (the buffer descriptor ends with the tile's last row: rows behind it read as
+// zero).  Row r is 128 bytes, its 16-byte piece c at place c ^ ((r >> 1) & 7), so that the same piece of any 16 consecutive rows lies on
+// different banks.  A step multiplies one block in two halves of 64, and the fragments of a half are read from LDS while the half before it is
+// multiplied, so the matrix unit waits for nothing but the one barrier of a step: behind it everyone has read the block, whose place the block after
+// the next is then loaded into.  With one wave on each SIMD there is nobody else to fill a gap, hence the interleaving by hand (weave): one
+// LDS read and one load beside each matrix instruction.
+//
+// EXACT: the 8-bit matrix instructions add the products of one instruction with about 17 bits (measured: 1.6e-5 of the result for normal values,
+// 5.6e-5 for log-normal ones, against 1e-7 of the bfloat16 instruction).  That is below half a step of a 16-bit result (2^-9, 2^-12), and not what a
+// 32-bit one should carry: for those the codes are widened to bfloat16 on the way out of LDS.
+template <typename T, bool EXACT, int TM, int TN>
+__device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
+    constexpr int BM = 64 * TM, BN = 64 * TN, LA = BM / 32, LB = BN / 32;      // 32 rows of 128 bytes a load of the workgroup
+    __shared__ __align__(16) uint8_t a0[BM * 128], a1[BM * 128], b0[BN * 128], b1[BN * 128];      // four arrays: the compiler tells them apart
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave >> 1, wc = wave & 1;
+
+    // Workgroups go to the 8 XCDs in turn.  Each XCD gets a contiguous range of tiles, walked in bands of 8 rows of tiles, so that what its
+    // workgroups read at one time is a few rows and columns of tiles, in its own L2.
+    uint32_t tile_m, tile_n;
+    {
+        const uint32_t total = d.tiles_m * d.tiles_n, xcd = blockIdx.x & 7, full = total / 8, rest = total % 8;
+        const uint32_t t = xcd * full + min(xcd, rest) + (blockIdx.x >> 3), band = t / (8 * d.tiles_n), in = t % (8 * d.tiles_n);
+        const uint32_t high = min(8u, d.tiles_m - band * 8);
+        tile_m = band * 8 + in % high;
+        tile_n = in / high;
+    }
+    const uint64_t m0 = (uint64_t)tile_m * BM, n0 = (uint64_t)tile_n * BN;
+    const uint32_t kb0 = blockIdx.y * d.per_split, nb = min(d.blocks, kb0 + d.per_split) - kb0, width = d.blocks * 128;
+
+    auto buffer = [&](const uint8_t* codes, uint64_t row0, uint32_t rows, uint32_t tile) {
+        const uint64_t have = (uint64_t)min(tile, rows - (uint32_t)row0) * width - (uint64_t)kb0 * 128;
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(codes + row0 * width + (uint64_t)kb0 * 128), 0, (int)(uint32_t)have, 0x00027000);
+    };
+    const auto ra = buffer(d.a.codes, m0, d.m, BM), rb = buffer(d.b.codes, n0, d.n, BN);
+    const uint32_t r8 = wave * 8 + (lane >> 3);      // the row of the first load; the others' differ by multiples of 32 and swizzle alike
+    const uint32_t off = r8 * width + (((lane & 7) ^ ((r8 >> 1) & 7)) << 4);
+    auto load = [&](uint8_t* A, uint8_t* B, uint32_t kb) __attribute__((always_inline)) {
+        // The row goes into the offset that the descriptor's bound is held against, the block into the one that is not: a row behind the last is out
+        // of bounds by itself.  Behind the last block: that one again, for nobody.
+        const uint32_t at = min(kb, nb - 1) * 128;
+#pragma unroll
+        for (int i = 0; i < LA; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_t*)(A + (i * 4 + wave) * 1024), 16, off + i * 32 * width, at, 0, 0);
+#pragma unroll
+        for (int i = 0; i < LB; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_t*)(B + (i * 4 + wave) * 1024), 16, off + i * 32 * width, at, 0, 0);
+    };
+
+    // Scales: a byte for each row of a fragment, read two steps before it is used.
+    const uint64_t step_a = d.a.step(), step_b = d.b.step();
+    const uint8_t *sa = d.a.scales + d.a.at(m0) + kb0 * step_a, *sb = d.b.scales + d.b.at(n0) + kb0 * step_b;
+    uint32_t ca[TM], cb[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) ca[i] = (uint32_t)d.a.at(min((uint32_t)((wr * TM + i) * 32 + (lane & 31)), (uint32_t)(d.m - 1 - m0)));
+#pragma unroll
+    for (int i = 0; i < TN; ++i) cb[i] = (uint32_t)d.b.at(min((uint32_t)((wc * TN + i) * 32 + (lane & 31)), (uint32_t)(d.n - 1 - n0)));
+    auto scales = [&](int* p, int* q, uint32_t kb) __attribute__((always_inline)) {
+        const uint32_t at = min(kb, nb - 1);
+        const uint8_t *u = sa + at * step_a, *v = sb + at * step_b;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) p[i] = u[ca[i]];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) q[i] = v[cb[i]];
+    };
+
+    // Fragments: lane l holds row l % 32 and 32 of the half's 64 codes, the pieces 4 half + 2 (l / 32) and the next.
+    uint32_t pa[4], pb[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int piece = (((q >> 1) * 4 + (lane >> 5) * 2 + (q & 1)) ^ ((lane >> 1) & 7)) << 4;
+        pa[q] = (wr * TM * 32 + (lane & 31)) * 128 + piece;
+        pb[q] = (wc * TN * 32 + (lane & 31)) * 128 + piece;
+    }
+    auto fragment = [&](const uint8_t* base, uint32_t lo, uint32_t hi) __attribute__((always_inline)) {
+        const i32x4 x = *reinterpret_cast<const i32x4*>(base + lo), y = *reinterpret_cast<const i32x4*>(base + hi);
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto read = [&](const uint8_t* A, const uint8_t* B, int half, i32x8* fa, i32x8* fb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) fb[i] = fragment(B + i * 4096, pb[half * 2], pb[half * 2 + 1]);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[i] = fragment(A + i * 4096, pa[half * 2], pa[half * 2 + 1]);
+    };
+
+    f32x16 acc[TM][TN];      // transposed: b's rows in the registers, a's in the lanes, so that a lane holds neighbours of a row of the result
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int k = 0; k < TN; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.0f;
+    auto multiply = [&](const i32x8* fa, const i32x8* fb, const int* p, const int* q) __attribute__((always_inline)) {
+        if constexpr (EXACT) {
+            bf16x8 wb[TN][4];
+#pragma unroll
+            for (int k = 0; k < TN; ++k)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) wb[k][s] = widen8(fb[k][2 * s], fb[k][2 * s + 1], scale_value(q[k]));
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const bf16x8 wa = widen8(fa[i][2 * s], fa[i][2 * s + 1], scale_value(p[i]));
+#pragma unroll
+                    for (int k = 0; k < TN; ++k) acc[i][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[k][s], wa, acc[i][k], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int k = 0; k < TN; ++k)
+                    acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[k], fa[i], acc[i][k], 0, 0, 0, q[k], 0, p[i]);
+        }
+    };
+    auto weave = [&](bool loads) __attribute__((always_inline)) {
+        constexpr int MF = TM * TN * (EXACT ? 4 : 1), DS = 2 * (TM + TN), LD = LA + LB;
+        constexpr int per_ds = DS > MF ? DS / MF : 1, per_ld = LD > MF ? LD / MF : 1;
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                    // a matrix instruction,
+            if (loads) __builtin_amdgcn_sched_group_barrier(0x010, per_ld, 0);    // a load,
+            __builtin_amdgcn_sched_group_barrier(0x100, per_ds, 0);               // a read from LDS
+        }
+    };
+
+    i32x8 fa0[TM], fb0[TN], fa1[TM], fb1[TN];
+    int xa[TM], xb[TN], ya[TM], yb[TN], nxa[TM], nxb[TN], nya[TM], nyb[TN];
+    auto step = [&](uint8_t* A, uint8_t* B, const uint8_t* A2, const uint8_t* B2, const int* p, const int* q, uint32_t kb) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0): the first half's fragments
+        GF_FENCE;
+        read(A, B, 1, fa1, fb1);
+        multiply(fa0, fb0, p, q);
+        weave(false);
+        GF_FENCE;
+        __builtin_amdgcn_s_waitcnt(0x0070);      // vmcnt(0), lgkmcnt(0): the next block is there, and this one is read
+        __builtin_amdgcn_s_barrier();
+        GF_FENCE;
+        load(A, B, kb + 2);
+        read(A2, B2, 0, fa0, fb0);
+        multiply(fa1, fb1, p, q);
+        weave(true);
+        GF_FENCE;
+    };
+    auto rotate = [&](uint32_t kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) { xa[i] = nxa[i]; ya[i] = nya[i]; }
+#pragma unroll
+        for (int i = 0; i < TN; ++i) { xb[i] = nxb[i]; yb[i] = nyb[i]; }
+        scales(nxa, nxb, kb + 2);
+        scales(nya, nyb, kb + 3);
+        GF_FENCE;
+    };
+    load(a0, b0, 0);
+    scales(nxa, nxb, 0);
+    scales(nya, nyb, 1);
+    load(a1, b1, 1);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __builtin_amdgcn_s_barrier();
+    GF_FENCE;
+    read(a0, b0, 0, fa0, fb0);
+    uint32_t kb = 0;
+    for (; kb + 1 < nb; kb += 2) {
+        rotate(kb);
+        step(a0, b0, a1, b1, xa, xb, kb);
+        step(a1, b1, a0, b0, ya, yb, kb + 1);
+    }
+    if (nb & 1) {
+        rotate(kb);
+        read(a0, b0, 1, fa1, fb1);
+        multiply(fa0, fb0, xa, xb);
+        multiply(fa1, fb1, xa, xb);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);      // no load is under way and nobody reads any more: LDS is free
+    __builtin_amdgcn_s_barrier();
+
+    // 32 rows of the wave's part at a time through LDS, so that a row leaves in pieces of 16 bytes.
+    constexpr int COLS = 32 * TN, PITCH = COLS * (int)sizeof(T) + 16, EACH = 16 / (int)sizeof(T), PIECES = COLS / EACH;
+    static_assert(32 * PITCH <= BN * 128 && 32 * PITCH <= BM * 128, "staging");
+    uint8_t* mine = wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1;
+    T* out = (T*)d.out + (uint64_t)blockIdx.y * d.m * d.n;
+    const bool wide = ((uint64_t)d.n * sizeof(T)) % 16 == 0;      // (the output starts at a multiple of 16 bytes)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int k = 0; k < TN; ++k)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float v[4] = {acc[i][k][4 * g], acc[i][k][4 * g + 1], acc[i][k][4 * g + 2], acc[i][k][4 * g + 3]};
+                store4((T*)(mine + (lane & 31) * PITCH) + k * 32 + g * 8 + (lane >> 5) * 4, v);
+            }
+        __builtin_amdgcn_s_waitcnt(0xc07f);      // the wave's own stores (it alone reads them)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 32 * PIECES / 64; ++q) {
+            const int r = (q * 64 + lane) / PIECES, c = (q * 64 + lane) % PIECES;
+            const uint64_t row = m0 + (wr * TM + i) * 32 + r, col = n0 + wc * COLS + c * EACH;
+            const i32x4 v = *reinterpret_cast<const i32x4*>(mine + r * PITCH + c * 16);
+            if (row >= d.m || col >= d.n) continue;
+            T* to = out + row * d.n + col;
+            if (wide) {
+                *reinterpret_cast<i32x4*>(to) = v;
+            } else {
+                const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+                for (int k = 0; k < EACH; ++k) if (col + k < d.n) to[k] = e[k];
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <typename T, bool EXACT, int TM, int TN>
+__global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN>(d); }
+
+// out = the sum of the splits' parts, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(const float* part, uint32_t splits, uint64_t count, T* out) {
+    const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= count) return;
+    const int left = (int)min((uint64_t)4, count - i);
+    const bool wide = count % 4 == 0;
+    float s[4] = {0, 0, 0, 0};
+    for (uint32_t k = 0; k < splits; ++k) {
+        float v[4];
+        load4_of(part + k * count + i, left, wide, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+    store4_of(out + i, left, true, s);
+}
+
+// ---- a few rows ----------------------------------------------------------------------------------------------------------------------------
+// The weight's bytes bound it.  A wave takes 16 rows of the weight (one row of codes is 128 bytes a block: whole cache lines, straight into registers) and
+// every WAVES-th block; it brings the same block of x to 8 bits itself, in the registers that the matrix instruction takes it from: lane l holds row
+// l % 16 of x, values (l / 16) * 32 .. + 31 of the block, so the block's largest magnitude is two exchanges away.
+constexpr int kRowWaves = 8;
+
+template <typename T>
+__global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d, const int wide) {
+    __shared__ f32x4 part[kRowWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const uint64_t n0 = (uint64_t)blockIdx.x * 16, blocks = (d.k + 127) / 128;
+    const uint64_t row = min(n0 + r, d.n - 1);
+    const uint8_t* w = d.codes + row * blocks * 128 + q * 32;
+    const uint8_t* ws = d.scales + (row >> 7) * blocks;
+    const T* x = (const T*)d.x + min((uint64_t)r, d.m - 1) * d.ldx;
+    f32x4 acc = {0, 0, 0, 0};
+    for (uint64_t b = wave; b < blocks; b += kRowWaves) {
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(w + b * 128), hi = *reinterpret_cast<const i32x4*>(w + b * 128 + 16);
+        const int sw = ws[b];
+        float v[32];
+        const uint64_t k0 = b * 128 + q * 32;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint64_t k = k0 + 4 * i;
+            const int left = (uint32_t)r < d.m && k < d.k ? (int)min((uint64_t)4, d.k - k) : 0;
+            load4_of(x + (left ? k : 0), left, wide, v + 4 * i);
+        }
+        uint32_t a = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) a = max(a, abs_bits(v[i]));
+        a = max(a, (uint32_t)__shfl_xor((int)a, 16));
+        a = max(a, (uint32_t)__shfl_xor((int)a, 32));
+        const uint32_t sx = scale_byte(a);
+        const float inv = scale_inverse(sx);
+        i32x8 fx;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fx[i] = (int)encode4(v + 4 * i, inv);
+        if constexpr (sizeof(T) == 4) {      // a 32-bit result: see EXACT above
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const i32x4 part = i < 2 ? lo : hi;
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(part[2 * (i & 1)], part[2 * (i & 1) + 1], scale_value(sw)),
+                                                              widen8(fx[2 * i], fx[2 * i + 1], scale_value((int)sx)), acc, 0, 0, 0);
+            }
+        } else {
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), fx, acc, 0, 0, 0, sw, 0, (int)sx);
+        }
+    }
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (threadIdx.x >= 256) return;
+    const int e = threadIdx.x & 3, l = threadIdx.x >> 2;      // part[.][l][e]: row l % 16 of x, row 4 (l / 16) + e of the weight
+    float s = 0;
+#pragma unroll
+    for (int k = 0; k < kRowWaves; ++k) s += part[k][l][e];
+    const uint64_t m = l & 15, n = n0 + 4 * (l >> 4) + e;
+    if (m < d.m && n < d.n) ((T*)d.out)[m * d.n + n] = (T)s;
+}
+
+// The tile's edge and how many ways the sum over K is split.  Tiles of 256 x 256 read half the bytes from LDS and L2 per product that those of
+// 128 x 128 do and are taken where there are enough of them to give every CU one; otherwise 128, of which two fit a CU, and the sum is split until
+// every CU has work, with at least four blocks of 128 in each split.
+struct Plan { uint32_t edge, tiles_m, tiles_n, splits, per_split; };
+
+static Plan plan_of(uint64_t m, uint64_t n, uint64_t blocks) {
+    Plan p;
+    auto tiles = [&](uint64_t edge) { return ((m + edge - 1) / edge) * ((n + edge - 1) / edge); };
+    p.edge = tiles(256) >= 192 ? 256 : 128;
+    p.tiles_m = (uint32_t)((m + p.edge - 1) / p.edge);
+    p.tiles_n = (uint32_t)((n + p.edge - 1) / p.edge);
+    const uint64_t t = tiles(p.edge);
+    uint64_t s = t >= 256 || p.edge == 256 ? 1 : 512 / t;
+    if (s > blocks / 4) s = blocks / 4;
+    if (s < 1) s = 1;
+    p.per_split = (uint32_t)((blocks + s - 1) / s);
+    p.splits = (uint32_t)((blocks + p.per_split - 1) / p.per_split);      // none of them empty
+    return p;
+}
+
+template <typename T, bool EXACT>
+static void launch_tiles(const MatmulArgs& a, const Plan& p, hipStream_t s) {
+    const dim3 grid(p.tiles_m * p.tiles_n, p.splits);
+    if (p.edge == 256) k_matmul<T, EXACT, 4, 4><<<grid, 256, 0, s>>>(a);
+    else k_matmul<T, EXACT, 2, 2><<<grid, 256, 0, s>>>(a);
+}
+
+template <typename T>
+static void launch_matmul(MatmulArgs a, const Plan& p, void* workspace, hipStream_t s) {
+    constexpr bool exact = sizeof(T) == 4;
+    if (p.splits == 1) { launch_tiles<T, exact>(a, p, s); return; }
+    T* out = (T*)a.out;
+    a.out = workspace;
+    launch_tiles<float, exact>(a, p, s);
+    const uint64_t count = (uint64_t)a.m * a.n;
+    k_join<T><<<(uint32_t)((count + 1023) / 1024), 256, 0, s>>>((const float*)workspace, p.splits, count, out);
+}
+
+static const char* operand_error(const gf_fp8_operand_t& o, uint64_t rows) {
+    if (!o.codes || !o.scales) return "null operand";
+    if ((uintptr_t)o.codes % 16) return "codes must start at a multiple of 16 bytes";
+    if (o.pitch && o.pitch < rows) return "scale pitch smaller than the rows";
+    if (!o.pitch && o.stride_row >> 24) return "scale stride too large";
+    return nullptr;
+}
+
+static bool too_large(uint64_t m, uint64_t n, uint64_t blocks) {      // blocks: a tile's rows have to lie within 4 GB
+    return m >> 31 || n >> 31 || blocks > 65535 || ((m + 127) / 128) * ((n + 127) / 128) >> 31 || (m * n) >> 41;
+}
+
+}  // namespace gf
+
+using namespace gf;
+
+GF_EXPORT uint64_t gf_fp8_matmul_workspace_bytes(uint64_t m, uint64_t n, uint64_t blocks) {
+    if (!m || !n || !blocks || too_large(m, n, blocks)) return 0;
+    const Plan p = plan_of(m, n, blocks);
+    return p.splits > 1 ? 4ull * p.splits * m * n : 0;
+}
+
+GF_EXPORT int gf_fp8_matmul(const gf_fp8_matmul_t* d, void* stream) {
+    if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null descriptor");
+    if (d->m == 0 || d->n == 0) return GF_OK;
+    if (!d->out) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null output");
+    if ((uintptr_t)d->out % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: the output must start at a multiple of 16 bytes");
+    if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: unknown dtype %u", d->dtype);
+    if (d->blocks == 0) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: no blocks to add up");
+    if (const char* e = operand_error(d->a, d->m)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: a: %s", e);
+    if (const char* e = operand_error(d->b, d->n)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: b: %s", e);
+    if (too_large(d->m, d->n, d->blocks)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: matrix too large (at most 65535 blocks along the sum)");
+    const Plan p = plan_of(d->m, d->n, d->blocks);
+    if (p.splits > 1 && (!d->workspace || (uintptr_t)d->workspace % 16)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null or unaligned workspace");
+    MatmulArgs a;
+    a.a = {d->a.codes, d->a.scales, d->a.pitch, d->a.stride_row, d->a.stride_block};
+    a.b = {d->b.codes, d->b.scales, d->b.pitch, d->b.stride_row, d->b.stride_block};
+    a.m = (uint32_t)d->m; a.n = (uint32_t)d->n; a.blocks = (uint32_t)d->blocks;
+    a.per_split = p.per_split; a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n;
+    a.out = d->out;
+    const hipStream_t s = gf_stream(stream);
+    if (d->dtype == F32) launch_matmul<float>(a, p, d->workspace, s);
+    else if (d->dtype == BF16) launch_matmul<__bf16>(a, p, d->workspace, s);
+    else launch_matmul<_Float16>(a, p, d->workspace, s);
+    return gf_check_launch("gf_fp8_matmul");
+}
+
+GF_EXPORT int gf_fp8_rows(const gf_fp8_rows_t* d, void* stream) {
+    if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: null descriptor");
+    if (d->m == 0 || d->n == 0) return GF_OK;
+    if (!d->x || !d->codes || !d->scales || !d->out) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: null pointer");
+    if (d->m > 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: at most 16 rows, got %llu", (unsigned long long)d->m);
+    if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: unknown dtype %u", d->dtype);
+    if (d->k == 0 || d->ldx < d->k) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: ldx < k, or k = 0");
+    if ((uintptr_t)d->codes % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: codes must start at a multiple of 16 bytes");
+    if ((d->n + 15) / 16 >> 31) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: matrix too large");
+    const uint64_t size = d->dtype == F32 ? 4 : 2;
+    const int wide = ((uintptr_t)d->x | d->ldx * size) % (4 * size) == 0;
+    const uint32_t grid = (uint32_t)((d->n + 15) / 16);
+    const hipStream_t s = gf_stream(stream);
+    if (d->dtype == F32) k_rows<float><<<grid, 64 * kRowWaves, 0, s>>>(*d, wide);
+    else if (d->dtype == BF16) k_rows<__bf16><<<grid, 64 * kRowWaves, 0, s>>>(*d, wide);
+    else k_rows<_Float16><<<grid, 64 * kRowWaves, 0, s>>>(*d, wide);
+    return gf_check_launch("gf_fp8_rows");
+}

@@ -74,6 +74,67 @@ typedef struct {
 uint64_t gf_grad_norm_workspace_bytes(uint32_t count);
 int gf_grad_norm(const gf_grad_norm_t* desc, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Products of block-scaled 8-bit values.
+ *
+ * Codes are e4m3 (largest 448).  A block of 128 values has the scale 2^(byte - 127): the smallest power of two >= 2^-127 with
+ * (largest magnitude) <= 448 * scale; the byte is 255 and every code NaN where the block holds an infinity or a NaN.  Codes are
+ * rounded to nearest even.  An operand [R, K] that is summed over K is held as codes [R, Kp], Kp = K rounded up to a multiple of 128 and the
+ * codes behind K zero, and scales either by row, byte (r, b) at [b * pitch + r], or by tile of 128 x 128, byte at [(r / 128) * stride_row + b *
+ * stride_block].
+ * ---------------------------------------------------------------------------------------------- */
+
+/* src [rows, cols] of `dtype`, ld values from row to row.  row_codes [rows, up(cols)] with row_scales [up(cols)/128, row_pitch]: blocks along the
+ * rows; col_codes [cols, up(rows)] with col_scales [up(rows)/128, col_pitch]: blocks along the columns, transposed.  Either may be NULL.
+ * tiles != 0: one scale for each 128 x 128 in tile_scales [up(rows)/128, up(cols)/128] for both, row_scales and col_scales unused. */
+typedef struct {
+    const void* src;
+    uint64_t rows, cols, ld;
+    uint32_t dtype;
+    uint32_t tiles;
+    uint8_t* row_codes;
+    uint8_t* row_scales;
+    uint8_t* col_codes;
+    uint8_t* col_scales;
+    uint8_t* tile_scales;
+    uint64_t row_pitch, col_pitch;
+} gf_fp8_quantize_t;
+int gf_fp8_quantize(const gf_fp8_quantize_t* desc, void* stream);
+
+/* One operand of gf_fp8_matmul: codes [rows, 128 * blocks].  pitch > 0: scales by row; 0: by tile. */
+typedef struct {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    uint64_t pitch;
+    uint64_t stride_row, stride_block;
+} gf_fp8_operand_t;
+
+/* out [m, n] of `dtype` (contiguous, at a multiple of 16 bytes) = a [m, 128 blocks] b [n, 128 blocks]^T, added up in 32 bits; blocks <= 65535.
+ * workspace: gf_fp8_matmul_workspace_bytes(m, n, blocks) device bytes of this call's own (NULL where that is 0). */
+typedef struct {
+    gf_fp8_operand_t a, b;
+    uint64_t m, n, blocks;
+    void* out;
+    uint32_t dtype;
+    uint32_t _pad;
+    void* workspace;
+} gf_fp8_matmul_t;
+uint64_t gf_fp8_matmul_workspace_bytes(uint64_t m, uint64_t n, uint64_t blocks);
+int gf_fp8_matmul(const gf_fp8_matmul_t* desc, void* stream);
+
+/* out [m, n] = Q(x) w^T for m <= 16 rows x [m, k] of `dtype` (ldx values from row to row): x is brought to 8 bits on the way, w is held as codes
+ * [n, up(k)] with one scale for each 128 x 128 at [(n / 128) * ceil(k / 128) + k / 128].  out: `dtype`, contiguous. */
+typedef struct {
+    const void* x;
+    uint64_t m, n, k, ldx;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    void* out;
+    uint32_t dtype;
+    uint32_t _pad;
+} gf_fp8_rows_t;
+int gf_fp8_rows(const gf_fp8_rows_t* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
