@@ -51,7 +51,7 @@ TRAIN_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wn
 
 
 def train_sources():
-    return sorted(glob.glob(os.path.join(TRAIN_DIR, "*.hip")))
+    return sorted(glob.glob(os.path.join(TRAIN_DIR, "*.hip")) + glob.glob(os.path.join(TRAIN_DIR, "*.cpp")))
 
 
 def train_headers():

@@ -24,10 +24,16 @@ struct AdamwArgs {
     const float* grad_scale;
     const float* found_inf;
     const float* grad_norm;
-    uint32_t count;
-    uint32_t count_steps;                 // 1: every tensor has one workgroup, which counts its step itself
+    uint32_t count_steps;                 // 1: every tensor of the call has one workgroup, which counts its step itself
 };
 static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
+
+struct StepArgs {
+    float* step[496];
+    const float* found_inf;
+    uint32_t count;
+};
+static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
 
 struct Hyper { float shrink, om_beta1, beta2, om_beta2, rate, inv_root, eps, grad; };
 
@@ -103,13 +109,13 @@ __device__ __forceinline__ void step32(const gf_adamw_tensor_t& t, const Hyper& 
 constexpr uint32_t kDitherIndex = 3242174889u, kDitherStep = 2447445414u;     // 2^32 / rho, 2^32 / rho^2; rho the real root of x^3 = x + 1
 constexpr float kTiny = 7.888609052210118e-31f;                                // 2^-100
 
-// |y| <= 448 to its e4m3 code without the sign.  u20: the dither, 20 bits: as many as a 32-bit value has below the three that e4m3 keeps.
-__device__ __forceinline__ uint32_t encode_e4m3(float y, uint32_t u20) {
-    const uint32_t b = __float_as_uint(y);
-    const uint32_t normal = min(((b + u20) >> 20) - (120u << 3), 0x7eu);
-    const uint32_t small = (uint32_t)(y * 512.0f + (float)u20 * 0x1p-20f);     // below 2^-6 the spacing is 2^-9
-    const uint32_t code = b < 0x3c800000u ? small : normal;
-    return b > 0x7f800000u ? 0x7fu : code;                                     // not a number
+// Four values with |y| <= 448 to their e4m3 codes.  v_cvt_sr_fp8_f32 adds the top 20 bits of its seed below the three fraction bits that stay and
+// truncates, at values below 2^-6 the same at their spacing of 2^-9: floor(|y| / spacing + u), for every u and y (compared over 4 M pairs).
+__device__ __forceinline__ uint32_t encode_dithered4(const float y[4], uint32_t seed) {
+    int w = __builtin_amdgcn_cvt_sr_fp8_f32(y[0], (int)seed, 0, 0);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(y[1], (int)(seed + kDitherIndex), w, 1);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(y[2], (int)(seed + 2 * kDitherIndex), w, 2);
+    return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(y[3], (int)(seed + 3 * kDitherIndex), w, 3);
 }
 
 __device__ __forceinline__ void decode4(uint32_t w, float scale, float out[4]) {
@@ -153,35 +159,32 @@ __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h
             decode4(load_codes(m + at, left[q], wide), ms, fm + 4 * q);
             decode4(load_codes(v + at, left[q], wide), vs, fr + 4 * q);
         }
-        uint32_t am = 0, ar = 0;
+        float am = 0, ar = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 8; ++k) {      // (values that are not there are zeros and stay so)
             const float x = fg[k] * h.grad;
             fm[k] = moment1(h, fm[k], x);
-            fr[k] = sqrtf(moment2(h, fr[k] * fr[k], x));
-            fp[k] = updated(h, fp[k], fm[k], fr[k]);
-            const bool there = (k & 3) < left[k >> 2];
-            am = max(am, there ? abs_bits(fm[k]) : 0u);
-            ar = max(ar, there ? abs_bits(fr[k]) : 0u);
+            // square root and reciprocal to one unit in the last place: correctly rounded ones cost as much again as all else here
+            fr[k] = __builtin_amdgcn_sqrtf(moment2(h, fr[k] * fr[k], x));
+            fp[k] = fp[k] * h.shrink - h.rate * fm[k] * __builtin_amdgcn_rcpf(fr[k] * h.inv_root + h.eps);
+            am = max_abs(am, fm[k]);
+            ar = max_abs(ar, fr[k]);
         }
         // as integers: what is no number stays the largest and makes the whole block none
-        const uint32_t bm = row_max_u32(am), br = row_max_u32(ar);
-        const float a_m = bm > 0x7f800000u ? __uint_as_float(bm) : fmaxf(__uint_as_float(bm), kTiny);
-        const float a_r = br > 0x7f800000u ? __uint_as_float(br) : fmaxf(__uint_as_float(br), kTiny);
+        const uint32_t bm = row_max_u32(__float_as_uint(am)), br = row_max_u32(__float_as_uint(ar));
+        const float a_m = max_abs(kTiny, __uint_as_float(bm)), a_r = max_abs(kTiny, __uint_as_float(br));
         const float inv_m = 448.0f / a_m, inv_r = 448.0f / a_r;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            uint32_t wm = 0, wr = 0;
+            const uint32_t seed = (uint32_t)(i0 + 64 * q) * kDitherIndex + word;
+            float ym[4], yr[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t u = ((uint32_t)(i0 + 64 * q + k) * kDitherIndex + word) >> 12;
-                const float fm_ = fm[4 * q + k], fr_ = fr[4 * q + k];
-                const uint32_t cm = encode_e4m3(fabsf(fm_ * inv_m), u) | ((__float_as_uint(fm_) >> 24) & 0x80u);
-                uint32_t cr = encode_e4m3(fr_ * inv_r, u ^ 0x80000u);
-                cr = (cr == 0 && fr_ > 0.0f) ? 1u : cr;      // a second moment above zero stays so: m / sqrt(v) must not meet a lost one
-                wm |= cm << (8 * k);
-                wr |= cr << (8 * k);
+                ym[k] = __builtin_amdgcn_fmed3f(fm[4 * q + k] * inv_m, -448.0f, 448.0f);
+                // a second moment above zero stays so (the smallest code is 2^-9): m / sqrt(v) must not meet a lost one
+                yr[k] = __builtin_amdgcn_fmed3f(fr[4 * q + k] * inv_r, fr[4 * q + k] > 0.0f ? 0x1p-9f : 0.0f, 448.0f);
             }
+            const uint32_t wm = encode_dithered4(ym, seed), wr = encode_dithered4(yr, seed ^ 0x80000000u);
             if (left[q]) {
                 const uint64_t i = i0 + 64 * q;
                 store_codes(m + i, wm, left[q], wide);
@@ -211,10 +214,10 @@ __global__ __launch_bounds__(kThreads) void k_adamw(const AdamwArgs a) {
     }
 }
 
-// The counts of tensors with several workgroups: raised when all of those have read them, i.e. by the next launch of the stream.
-__global__ void k_count_steps(const AdamwArgs a) {
+// The counts of a call in which a tensor has several workgroups: raised when all of those have read them, i.e. by a launch behind.
+__global__ __launch_bounds__(512) void k_count_steps(const StepArgs a) {
     if (a.found_inf && *a.found_inf != 0.0f) return;
-    if (threadIdx.x < a.count) *a.t[threadIdx.x].step += 1.0f;
+    if (threadIdx.x < a.count) *a.step[threadIdx.x] += 1.0f;
 }
 
 template <typename T>
@@ -305,13 +308,14 @@ GF_EXPORT int gf_adamw_step(const gf_adamw_t* d, void* stream) {
     if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: unknown dtype %u", d->dtype);
     if (d->state_bits != 32 && d->state_bits != 8) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: state_bits must be 32 or 8, got %u", d->state_bits);
     if (!(d->beta1 >= 0 && d->beta1 < 1 && d->beta2 >= 0 && d->beta2 < 1)) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: betas must be in [0, 1)");
-    uint64_t total = 0;
+    uint64_t total = 0, most = 0;
     for (uint32_t i = 0; i < d->count; ++i) {
         const gf_adamw_tensor_t& t = d->tensors_host[i];
         if (!t.step || (t.n && (!t.p || !t.g || !t.m || !t.v || (d->state_bits == 8 && (!t.m_scale || !t.v_scale)))))
             return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: null pointer in tensor %u", i);
         if (t.n >> 40) return gf_set_error(GF_ERR_INVALID, "gf_adamw_step: tensor %u has too many values", i);
         total += t.n;
+        most = t.n > most ? t.n : most;
     }
     // Values per workgroup: as many workgroups as keep the chip's 256 CUs busy where there is work for them, few enough that each amortises its
     // scalars (two powers in 64 bits, about half a microsecond) where there is more.
@@ -323,31 +327,34 @@ GF_EXPORT int gf_adamw_step(const gf_adamw_t* d, void* stream) {
     a.beta1 = d->beta1; a.beta2 = d->beta2; a.lr = d->lr;
     a.eps = (float)d->eps; a.weight_decay = (float)d->weight_decay; a.max_norm = (float)d->max_norm;
     a.chunk = chunk;
+    a.count_steps = most <= chunk;
     a.lr_device = d->lr_device; a.grad_scale = d->grad_scale; a.found_inf = d->found_inf; a.grad_norm = d->grad_norm;
     const uint32_t eb = elem_bytes(d->dtype), sb = d->state_bits / 8;
+    const hipStream_t s = gf_stream(stream);
     for (uint32_t i = 0; i < d->count;) {
         uint32_t k = 0, blocks = 0;
-        bool several = false;
         for (; i < d->count && k < kTensors; ++i, ++k) {
             gf_adamw_tensor_t t = d->tensors_host[i];
             const uint32_t need = t.n ? (uint32_t)((t.n + chunk - 1) / chunk) : 1;       // an empty tensor's step is counted too
-            several |= need > 1;
             if (off(t.p, 4 * eb) || off(t.g, 4 * eb) || off(t.m, 4 * sb) || off(t.v, 4 * sb)) t.n |= kNarrow;
             a.t[k] = t;
             a.first[k] = blocks;
             blocks += need;
         }
-        a.count = k;
-        a.count_steps = !several;
         for (; k < kTensors; ++k) { a.t[k] = a.t[0]; a.first[k] = 0xffffffffu; }
-        const hipStream_t s = gf_stream(stream);
         if (d->dtype == F32) launch_adamw<float>(a, blocks, d->state_bits, s);
         else if (d->dtype == BF16) launch_adamw<__bf16>(a, blocks, d->state_bits, s);
         else launch_adamw<_Float16>(a, blocks, d->state_bits, s);
-        if (several) k_count_steps<<<1, 64, 0, s>>>(a);
-        if (const int rc = gf_check_launch("gf_adamw_step")) return rc;
     }
-    return GF_OK;
+    if (!a.count_steps) {
+        StepArgs c;
+        c.found_inf = d->found_inf;
+        for (uint32_t i = 0; i < d->count;) {
+            for (c.count = 0; i < d->count && c.count < 496; ++i) c.step[c.count++] = d->tensors_host[i].step;
+            k_count_steps<<<1, 512, 0, s>>>(c);
+        }
+    }
+    return gf_check_launch("gf_adamw_step");
 }
 
 GF_EXPORT uint64_t gf_grad_norm_workspace_bytes(uint32_t count) { return 8ull * ((uint64_t)kNormBlocks + count); }

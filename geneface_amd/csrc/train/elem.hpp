@@ -50,6 +50,9 @@ __device__ __forceinline__ uint32_t row_max_u32(uint32_t x) {
     return x;
 }
 
+// largest magnitude; NaN where either is (v_maximum3_f32)
+__device__ __forceinline__ float max_abs(float a, float x) { return __builtin_elementwise_maximum(a, __builtin_fabsf(x)); }
+
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 }  // namespace gf

@@ -253,21 +253,35 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
 template <typename T, bool EXACT, int TM, int TN>
 __global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN>(d); }
 
-// out = the sum of the splits' parts, in their order
-template <typename T>
-__global__ __launch_bounds__(256) void k_join(const float* part, uint32_t splits, uint64_t count, T* out) {
-    const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= count) return;
-    const int left = (int)min((uint64_t)4, count - i);
+// out = the sum of the splits' parts in a fixed order: a wave adds up every WAVES-th of them for 256 values, then the waves' sums are added.  Eight
+// loads are under way at a time: the parts of a tall product's weight gradient are hundreds, of few values each, and latency is all they cost.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_join(const float* part, uint32_t splits, uint64_t count, T* out) {
+    __shared__ f32x4 sums[WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t i = ((uint64_t)blockIdx.x * 64 + lane) * 4;
+    const int left = i < count ? (int)min((uint64_t)4, count - i) : 0;
     const bool wide = count % 4 == 0;
-    float s[4] = {0, 0, 0, 0};
-    for (uint32_t k = 0; k < splits; ++k) {
-        float v[4];
-        load4_of(part + k * count + i, left, wide, v);
+    const float* at = part + (left ? i : 0);
+    f32x4 s = {0, 0, 0, 0};
+    for (uint32_t k = wave; k < splits; k += 8 * WAVES) {
+        float v[8][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
+        for (int u = 0; u < 8; ++u) load4_of(at + min(k + u * WAVES, splits - 1) * count, k + u * WAVES < splits ? left : 0, wide, v[u]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += v[u][e];
     }
-    store4_of(out + i, left, true, s);
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave) return;
+    float r[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] += sums[w][lane][e];
+    store4_of(out + (left ? i : 0), left, true, r);
 }
 
 // ---- a few rows ----------------------------------------------------------------------------------------------------------------------------
@@ -330,14 +344,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d, 
 }
 
 // The tile's edge and how many ways the sum over K is split.  Tiles of 256 x 256 read half the bytes from LDS and L2 per product that those of
-// 128 x 128 do and are taken where there are enough of them to give every CU one; otherwise 128, of which two fit a CU, and the sum is split until
+// 128 x 128 do and are taken where there are enough of them to give every CU one and they reach little further behind the last row and column;
+// otherwise 128, of which two fit a CU, and the sum is split until
 // every CU has work, with at least four blocks of 128 in each split.
 struct Plan { uint32_t edge, tiles_m, tiles_n, splits, per_split; };
 
 static Plan plan_of(uint64_t m, uint64_t n, uint64_t blocks) {
     Plan p;
     auto tiles = [&](uint64_t edge) { return ((m + edge - 1) / edge) * ((n + edge - 1) / edge); };
-    p.edge = tiles(256) >= 192 ? 256 : 128;
+    p.edge = tiles(256) >= 192 && 4 * tiles(256) <= tiles(128) + tiles(128) / 8 ? 256 : 128;
     p.tiles_m = (uint32_t)((m + p.edge - 1) / p.edge);
     p.tiles_n = (uint32_t)((n + p.edge - 1) / p.edge);
     const uint64_t t = tiles(p.edge);
@@ -364,7 +379,9 @@ static void launch_matmul(MatmulArgs a, const Plan& p, void* workspace, hipStrea
     a.out = workspace;
     launch_tiles<float, exact>(a, p, s);
     const uint64_t count = (uint64_t)a.m * a.n;
-    k_join<T><<<(uint32_t)((count + 1023) / 1024), 256, 0, s>>>((const float*)workspace, p.splits, count, out);
+    const uint32_t grid = (uint32_t)((count + 255) / 256);
+    if (p.splits > 16) k_join<T, 16><<<grid, 1024, 0, s>>>((const float*)workspace, p.splits, count, out);
+    else k_join<T, 4><<<grid, 256, 0, s>>>((const float*)workspace, p.splits, count, out);
 }
 
 static const char* operand_error(const gf_fp8_operand_t& o, uint64_t rows) {

@@ -21,7 +21,6 @@ from .lib import check, current_stream, lib
 from .optim import DTYPES
 
 BLOCK = 128
-FEW_ROWS = 16      # rows that gf_fp8_rows takes
 
 _vp = C.c_void_p
 
@@ -32,21 +31,17 @@ class GfFp8Quantize(C.Structure):
                [(n, _vp) for n in ("row_codes", "row_scales", "col_codes", "col_scales", "tile_scales")] + [("row_pitch", C.c_uint64), ("col_pitch", C.c_uint64)]
 
 
-class GfFp8Operand(C.Structure):
-    """ctypes mirror of gf_fp8_operand_t."""
-    _fields_ = [("codes", _vp), ("scales", _vp), ("pitch", C.c_uint64), ("stride_row", C.c_uint64), ("stride_block", C.c_uint64)]
+class GfFp8Linear(C.Structure):
+    """ctypes mirror of gf_fp8_linear_t."""
+    _fields_ = [("x", _vp), ("ldx", C.c_uint64), ("w", _vp), ("ldw", C.c_uint64), ("codes", _vp), ("scales", _vp), ("m", C.c_uint64), ("n", C.c_uint64),
+                ("k", C.c_uint64), ("y", _vp), ("saved", _vp), ("workspace", _vp)] + [(n, C.c_uint32) for n in ("dtype", "w_dtype", "keep_w", "keep_x")] + \
+               [(n, C.c_uint64) for n in ("saved_bytes", "workspace_bytes", "backward_bytes")]
 
 
-class GfFp8Matmul(C.Structure):
-    """ctypes mirror of gf_fp8_matmul_t."""
-    _fields_ = [("a", GfFp8Operand), ("b", GfFp8Operand), ("m", C.c_uint64), ("n", C.c_uint64), ("blocks", C.c_uint64), ("out", _vp),
-                ("dtype", C.c_uint32), ("_pad", C.c_uint32), ("workspace", _vp)]
-
-
-class GfFp8Rows(C.Structure):
-    """ctypes mirror of gf_fp8_rows_t."""
-    _fields_ = [("x", _vp), ("m", C.c_uint64), ("n", C.c_uint64), ("k", C.c_uint64), ("ldx", C.c_uint64), ("codes", _vp), ("scales", _vp), ("out", _vp),
-                ("dtype", C.c_uint32), ("_pad", C.c_uint32)]
+class GfFp8LinearBackward(C.Structure):
+    """ctypes mirror of gf_fp8_linear_backward_t."""
+    _fields_ = [("dy", _vp), ("lddy", C.c_uint64), ("saved", _vp), ("m", C.c_uint64), ("n", C.c_uint64), ("k", C.c_uint64), ("dx", _vp), ("dw", _vp),
+                ("workspace", _vp)] + [(n, C.c_uint32) for n in ("dtype", "w_dtype", "keep_w", "keep_x")]
 
 
 def _blocks(n):
@@ -55,7 +50,7 @@ def _blocks(n):
 
 def _matrix(x):
     """x [..., K] as [M, K] whose rows are consecutive values, rows at any distance."""
-    m = x.reshape(-1, x.shape[-1])
+    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     return m if m.stride(1) == 1 and m.stride(0) >= m.shape[1] else m.contiguous()
 
 
@@ -83,26 +78,6 @@ def _quantize(m, rows, cols, tiles=False):
                       None if tiles else p(cs), p(ts), R, Cn)
     check(lib().gf_fp8_quantize(C.byref(d), current_stream(m.device)))
     return rc, rs, cc, cs
-
-
-def _by_row(codes, scales):
-    return GfFp8Operand(codes.data_ptr(), scales.data_ptr(), scales.shape[1], 0, 0)
-
-
-def _by_tile(codes, scales, transposed=False):
-    """Scales [row block, block along the sum], or [block along the sum, row block] where the codes are the transposed ones."""
-    a, b = scales.stride(0), scales.stride(1)
-    return GfFp8Operand(codes.data_ptr(), scales.data_ptr(), 0, b if transposed else a, a if transposed else b)
-
-
-def _matmul(a, b, m, n, blocks, dtype, device):
-    out = torch.empty(m, n, dtype=dtype, device=device)
-    L = lib()
-    need = L.gf_fp8_matmul_workspace_bytes(m, n, blocks)
-    work = torch.empty(need // 4, dtype=torch.float32, device=device) if need else None
-    d = GfFp8Matmul(a, b, m, n, blocks, out.data_ptr(), DTYPES[dtype], 0, None if work is None else work.data_ptr())
-    check(L.gf_fp8_matmul(C.byref(d), current_stream(device)))
-    return out
 
 
 class Fp8Weight:
@@ -154,49 +129,64 @@ def quantize_weight(weight):
     return Fp8Weight(codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu), K)
 
 
-def _linear_packed(x, w):
-    K, N = w.in_features, w.out_features
-    if not (x.numel() and N):
-        return torch.zeros(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    m = _matrix(x)
-    M = m.shape[0]
-    with torch.cuda.device(x.device):
-        if M <= FEW_ROWS:
-            out = torch.empty(M, N, dtype=x.dtype, device=x.device)
-            d = GfFp8Rows(m.data_ptr(), M, N, K, m.stride(0) if M > 1 else K, w.values.data_ptr(), w.scales.data_ptr(), out.data_ptr(), DTYPES[x.dtype], 0)
-            check(lib().gf_fp8_rows(C.byref(d), current_stream(x.device)))
-        else:
-            codes, scales, _, _ = _quantize(m, True, False)
-            out = _matmul(_by_row(codes, scales), _by_tile(w.values, w.scales), M, N, _blocks(K), x.dtype, x.device)
-    return out.view(*x.shape[:-1], N)
+def _forward(x, w, packed, keep_w, keep_x):
+    """(y, what the backward pass needs, its workspace's bytes) of x [M, K] and w [N, K], on x's device."""
+    dev = x.device
+    M, K = x.shape
+    N = w.out_features if packed else w.shape[0]
+    d = GfFp8Linear(x.data_ptr(), x.stride(0) if M > 1 else K, m=M, n=N, k=K, dtype=DTYPES[x.dtype], keep_w=keep_w, keep_x=keep_x)
+    if packed:
+        d.codes, d.scales = w.values.data_ptr(), w.scales.data_ptr()
+    else:
+        d.w, d.ldw, d.w_dtype = w.data_ptr(), w.stride(0) if N > 1 else K, DTYPES[w.dtype]
+    L = lib()
+    check(L.gf_fp8_linear_plan(C.byref(d)))
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    saved = torch.empty(d.saved_bytes, dtype=torch.uint8, device=dev) if d.saved_bytes else None
+    work = torch.empty(d.workspace_bytes, dtype=torch.uint8, device=dev) if d.workspace_bytes else None
+    d.y, d.saved, d.workspace = y.data_ptr(), None if saved is None else saved.data_ptr(), None if work is None else work.data_ptr()
+    check(L.gf_fp8_linear(C.byref(d), current_stream(dev)))
+    return y, saved, d.backward_bytes
+
+
+class _on:
+    """torch.cuda.device(dev), entered only where it is not the current device already."""
+    def __init__(self, dev):
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight):
-        (N, K), m = weight.shape, _matrix(x)
-        M, need_x, need_w = m.shape[0], ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        with torch.cuda.device(x.device):
-            wr, ws, wc, _ = _quantize(_matrix(weight), True, need_x, tiles=True)
-            xr, xs, xc, xcs = _quantize(m, True, need_w)      # kept for the backward pass: x in 8 bits, not x
-            y = _matmul(_by_row(xr, xs), _by_tile(wr, ws), M, N, _blocks(K), x.dtype, x.device)
-        ctx.save_for_backward(wc, ws if need_x else None, xc, xcs)
-        ctx.sizes, ctx.dtypes = (M, N, K), (x.dtype, weight.dtype)
+        keep_w, keep_x = ctx.needs_input_grad
+        with _on(x.device):
+            y, saved, ctx.backward_bytes = _forward(_matrix(x), _matrix(weight), False, keep_w, keep_x)
+        ctx.save_for_backward(saved)      # w by columns and x by columns, in 8 bits: neither tensor itself
+        ctx.sizes, ctx.dtypes, ctx.keep = (*x.shape, weight.shape[0]), (x.dtype, weight.dtype), (keep_w, keep_x)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        wc, ws, xc, xcs = ctx.saved_tensors
-        (M, N, K), (tx, tw) = ctx.sizes, ctx.dtypes
-        need_x, need_w = ctx.needs_input_grad
-        dx = dw = None
-        with torch.cuda.device(dy.device):
-            gr, gs, gc, gcs = _quantize(_matrix(dy), need_x, need_w)
-            if need_x:
-                dx = _matmul(_by_row(gr, gs), _by_tile(wc, ws, transposed=True), M, K, _blocks(N), tx, dy.device)
-            if need_w:
-                dw = _matmul(_by_row(gc, gcs), _by_row(xc, xcs), N, K, _blocks(M), tw, dy.device)
+        saved, = ctx.saved_tensors
+        (M, K, N), (tx, tw), (keep_w, keep_x) = ctx.sizes, ctx.dtypes, ctx.keep
+        want_x, want_w = ctx.needs_input_grad
+        dev, dy = dy.device, _matrix(dy)
+        with _on(dev):
+            dx = torch.empty(M, K, dtype=tx, device=dev) if want_x else None
+            dw = torch.empty(N, K, dtype=tw, device=dev) if want_w else None
+            work = torch.empty(ctx.backward_bytes, dtype=torch.uint8, device=dev)
+            d = GfFp8LinearBackward(dy.data_ptr(), dy.stride(0) if M > 1 else N, saved.data_ptr(), M, N, K, dx.data_ptr() if want_x else None,
+                                    dw.data_ptr() if want_w else None, work.data_ptr(), DTYPES[tx], DTYPES[tw], keep_w, keep_x)
+            check(lib().gf_fp8_linear_backward(C.byref(d), current_stream(dev)))
         return dx, dw
 
 
@@ -222,7 +212,12 @@ def linear(x, weight):
     if packed:
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("fp8: an Fp8Weight has no backward pass: give the weight itself, or call under no_grad")
-        return _linear_packed(x, weight)
+        N = weight.out_features
+        if not (x.numel() and N):
+            return torch.zeros(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+        with _on(x.device):
+            y = _forward(_matrix(x), weight, True, False, False)[0]
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
     if not (x.numel() and weight.numel()):      # nothing to add up; differentiable
         return x @ weight.t().to(x.dtype)
     y = _Linear.apply(x.reshape(-1, K), weight)      # (a view made inside the node could not be written in place, as MLP's ReLU does)

@@ -135,6 +135,41 @@ typedef struct {
 } gf_fp8_rows_t;
 int gf_fp8_rows(const gf_fp8_rows_t* desc, void* stream);
 
+/* A linear layer, y [m, n] = Q_row(x) Q_tile(w)^T, and its gradients dx [m, k] = Q_row(dy) Q_tile(w), dw [n, k] = Q_col(dy)^T Q_col(x), each as one
+ * call that enqueues all its launches.  x, dy: ldx / lddy values from row to row.  The weight is given as values w [n, k] of w_dtype (ldw values from
+ * row to row), or as codes and scales as gf_fp8_rows takes them (w NULL).  y and dx have dtype, dw has w_dtype; all contiguous.
+ * keep_w, keep_x: what the backward call will need is left in `saved` (keep_w for dx: w by columns; keep_x for dw: x by columns, one byte a value).
+ * gf_fp8_linear_plan fills saved_bytes, workspace_bytes and backward_bytes (the workspace of the backward call); the buffers start at multiples of
+ * 256 bytes, and a workspace is one call's own until the stream has passed it.  No size may be 0. */
+typedef struct {
+    const void* x;
+    uint64_t ldx;
+    const void* w;
+    uint64_t ldw;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    uint64_t m, n, k;
+    void* y;
+    void* saved;
+    void* workspace;
+    uint32_t dtype, w_dtype, keep_w, keep_x;
+    uint64_t saved_bytes, workspace_bytes, backward_bytes;
+} gf_fp8_linear_t;
+int gf_fp8_linear_plan(gf_fp8_linear_t* desc_host);
+int gf_fp8_linear(const gf_fp8_linear_t* desc, void* stream);
+
+typedef struct {
+    const void* dy;
+    uint64_t lddy;
+    const void* saved;
+    uint64_t m, n, k;
+    void* dx;            /* NULL: not wanted (keep_w was 0 or the caller has no use for it) */
+    void* dw;            /* NULL: not wanted */
+    void* workspace;
+    uint32_t dtype, w_dtype, keep_w, keep_x;
+} gf_fp8_linear_backward_t;
+int gf_fp8_linear_backward(const gf_fp8_linear_backward_t* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -84,25 +84,48 @@ def test_the_library_refuses_bad_descriptors(hip_lib):
     refused(hip_lib.gf_fp8_quantize(q(ld=4), None), b"ld < cols")
     refused(hip_lib.gf_fp8_quantize(q(row_pitch=2), None), b"pitch")
     refused(hip_lib.gf_fp8_quantize(q(rows=1 << 40, cols=1 << 40, ld=1 << 40, row_pitch=1 << 40), None), b"too large")
-    op = lambda **k: fp8.GfFp8Operand(**{"codes": 16, "scales": 16, "pitch": 300, **k})      # noqa: E731
-    m = lambda **k: C.byref(fp8.GfFp8Matmul(**{"a": op(), "b": op(), "m": 300, "n": 300, "blocks": 2, "out": 16, **k}))      # noqa: E731
+    # gf_fp8_matmul_t as 64-bit words: a and b (codes, scales, pitch, stride of a tile's row and block), m, n, blocks, out, dtype, workspace
+    base = {"a_codes": 16, "a_scales": 16, "a_pitch": 300, "b_codes": 16, "b_scales": 16, "b_pitch": 300, "m": 300, "n": 300, "blocks": 2, "out": 16}
+    order = ["a_codes", "a_scales", "a_pitch", "a_row", "a_block", "b_codes", "b_scales", "b_pitch", "b_row", "b_block", "m", "n", "blocks", "out", "dtype", "workspace"]
+    m = lambda **k: (C.c_uint64 * 16)(*[{**base, **k}.get(n, 0) for n in order])      # noqa: E731
     refused(hip_lib.gf_fp8_matmul(None, None), b"null")
     assert hip_lib.gf_fp8_matmul(m(m=0), None) == 0 and hip_lib.gf_fp8_matmul(m(n=0), None) == 0
-    refused(hip_lib.gf_fp8_matmul(m(out=None), None), b"null output")
+    refused(hip_lib.gf_fp8_matmul(m(out=0), None), b"null output")
     refused(hip_lib.gf_fp8_matmul(m(out=8), None), b"multiple of 16")
     refused(hip_lib.gf_fp8_matmul(m(dtype=3), None), b"dtype")
     refused(hip_lib.gf_fp8_matmul(m(blocks=0), None), b"no blocks")
-    refused(hip_lib.gf_fp8_matmul(m(a=op(codes=None)), None), b"a: null")
-    refused(hip_lib.gf_fp8_matmul(m(b=op(scales=None)), None), b"b: null")
-    refused(hip_lib.gf_fp8_matmul(m(b=op(codes=24)), None), b"multiple of 16")
-    refused(hip_lib.gf_fp8_matmul(m(b=op(pitch=299)), None), b"pitch")
+    refused(hip_lib.gf_fp8_matmul(m(a_codes=0), None), b"a: null")
+    refused(hip_lib.gf_fp8_matmul(m(b_scales=0), None), b"b: null")
+    refused(hip_lib.gf_fp8_matmul(m(b_codes=24), None), b"multiple of 16")
+    refused(hip_lib.gf_fp8_matmul(m(b_pitch=299), None), b"pitch")
     refused(hip_lib.gf_fp8_matmul(m(blocks=1 << 16), None), b"too large")
     refused(hip_lib.gf_fp8_matmul(m(blocks=1000), None), b"workspace")
     assert hip_lib.gf_fp8_matmul_workspace_bytes(300, 300, 1000) % (4 * 300 * 300) == 0 and hip_lib.gf_fp8_matmul_workspace_bytes(300, 300, 1) == 0
-    r = lambda **k: C.byref(fp8.GfFp8Rows(**{"x": 16, "m": 3, "n": 7, "k": 5, "ldx": 5, "codes": 16, "scales": 16, "out": 16, **k}))      # noqa: E731
+    f = lambda **k: fp8.GfFp8Linear(**{"x": 16, "ldx": 5, "w": 16, "ldw": 5, "m": 300, "n": 7, "k": 5, "y": 16, "workspace": 256, "saved": 256, "keep_x": 1, **k})      # noqa: E731
+    refused(hip_lib.gf_fp8_linear_plan(None), b"null")
+    refused(hip_lib.gf_fp8_linear_plan(C.byref(f(k=0))), b"empty")
+    p = f(keep_w=1)
+    assert hip_lib.gf_fp8_linear_plan(C.byref(p)) == 0 and p.saved_bytes >= 5 * 128 + 1 + 5 * 384 + 15 and p.workspace_bytes >= 300 * 128 and p.backward_bytes >= 300 * 128 + 7 * 384
+    refused(hip_lib.gf_fp8_linear(None, None), b"null")
+    for change in (dict(x=None), dict(y=None), dict(w=None)):
+        refused(hip_lib.gf_fp8_linear(C.byref(f(**change)), None), b"null pointer")
+    refused(hip_lib.gf_fp8_linear(C.byref(f(n=0)), None), b"empty")
+    refused(hip_lib.gf_fp8_linear(C.byref(f(m=1 << 31)), None), b"too large")
+    refused(hip_lib.gf_fp8_linear(C.byref(f(saved=None)), None), b"null buffer")
+    refused(hip_lib.gf_fp8_linear(C.byref(f(workspace=16)), None), b"multiples of 256")
+    refused(hip_lib.gf_fp8_linear(C.byref(f(w=None, codes=16, scales=16)), None), b"no backward")
+    g = lambda **k: C.byref(fp8.GfFp8LinearBackward(**{"dy": 16, "lddy": 7, "saved": 256, "m": 300, "n": 7, "k": 5, "dx": 16, "dw": 16, "workspace": 256, "keep_w": 1, "keep_x": 1, **k}))      # noqa: E731
+    refused(hip_lib.gf_fp8_linear_backward(None, None), b"null")
+    assert hip_lib.gf_fp8_linear_backward(g(dx=None, dw=None), None) == 0
+    refused(hip_lib.gf_fp8_linear_backward(g(dy=None), None), b"null")
+    refused(hip_lib.gf_fp8_linear_backward(g(keep_x=0), None), b"not kept")
+    refused(hip_lib.gf_fp8_linear_backward(g(keep_w=0), None), b"not kept")
+    refused(hip_lib.gf_fp8_linear_backward(g(saved=16), None), b"multiples of 256")
+    rows = ["x", "m", "n", "k", "ldx", "codes", "scales", "out", "dtype"]
+    r = lambda **k: (C.c_uint64 * 9)(*[{**{"x": 16, "m": 3, "n": 7, "k": 5, "ldx": 5, "codes": 16, "scales": 16, "out": 16}, **k}.get(n, 0) for n in rows])      # noqa: E731
     refused(hip_lib.gf_fp8_rows(None, None), b"null")
     assert hip_lib.gf_fp8_rows(r(m=0), None) == 0
-    refused(hip_lib.gf_fp8_rows(r(x=None), None), b"null")
+    refused(hip_lib.gf_fp8_rows(r(x=0), None), b"null")
     refused(hip_lib.gf_fp8_rows(r(m=17), None), b"at most 16")
     refused(hip_lib.gf_fp8_rows(r(dtype=3), None), b"dtype")
     refused(hip_lib.gf_fp8_rows(r(k=0), None), b"k = 0")
