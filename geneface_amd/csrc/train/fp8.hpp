@@ -19,15 +19,129 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
     return e > 8 ? e - 8 : 0;
 }
 
-// 2^-(byte - 127), by which a block's values are multiplied (exactly); not a number where the block is none, so that all its codes are none too
-__device__ __forceinline__ float scale_inverse(uint32_t byte) {
-    return byte == kScaleNone ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - byte) << 23);
+// 2^(byte - 127), by which codes are multiplied and values divided.  255 gives infinity: the codes of a block that is none are NaN anyway
+__device__ __forceinline__ float scale_value(uint32_t byte) { return __uint_as_float(byte ? byte << 23 : 0x00400000u); }
+
+// all NaN where the block is none
+__device__ __forceinline__ uint2 coded(uint2 w, uint32_t byte) {
+    const uint32_t none = byte == kScaleNone ? 0x7f7f7f7fu : 0u;
+    return {w.x | none, w.y | none};
 }
 
-// four values to four codes, each rounded to nearest even once; |x * inverse| <= 448, so nothing saturates
-__device__ __forceinline__ uint32_t encode4(const float x[4], float inverse) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inverse, x[1] * inverse, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inverse, x[3] * inverse, w, true);
+// Eight consecutive values as they were loaded, and what is done to them in pairs: 16-bit values stay packed from memory to their codes.
+// v_cvt_scalef32_pk_fp8_* divides by a power of two and rounds to nearest even, once; |x| <= 448 * scale, so nothing saturates.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct Eight {      // 16-bit types
+    uint32_t w[4];
+    typedef T pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ i16x2 encode2(i16x2 into, uint32_t two, float scale, bool high);
+    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
+    __device__ __forceinline__ void load(const T* src, int left, int wide) {      // wide: 2: a multiple of 16 bytes, 1: of 8, 0: of 2
+        if (left >= 8 && wide == 2) { *reinterpret_cast<i32x4*>(w) = *reinterpret_cast<const i32x4*>(src); return; }
+        if (left >= 8 && wide == 1) {
+            *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+            *reinterpret_cast<uint2*>(w + 2) = *reinterpret_cast<const uint2*>(src + 4);
+            return;
+        }
+        const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (2 * i < left ? (uint32_t)s[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)s[2 * i + 1] << 16 : 0u);
+    }
+    // bits of a magnitude (as 16 bits) to those of the 32-bit value
+    static __device__ __forceinline__ uint32_t bits32(uint32_t h);
+    __device__ __forceinline__ uint32_t amax() const {
+        u16x2 m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+        return bits32(max((uint32_t)m[0], (uint32_t)m[1]));
+    }
+    __device__ __forceinline__ uint2 encode(float scale) const {
+        i16x2 lo = {0, 0}, hi = {0, 0};
+        lo = encode2(lo, w[0], scale, false); lo = encode2(lo, w[1], scale, true);
+        hi = encode2(hi, w[2], scale, false); hi = encode2(hi, w[3], scale, true);
+        return {__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    }
+};
+template <> __device__ __forceinline__ i16x2 Eight<__bf16>::encode2(i16x2 into, uint32_t two, float scale, bool high) {
+    const pair p = __builtin_bit_cast(pair, two);
+    return high ? __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(into, p, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(into, p, scale, false);
+}
+template <> __device__ __forceinline__ i16x2 Eight<_Float16>::encode2(i16x2 into, uint32_t two, float scale, bool high) {
+    const pair p = __builtin_bit_cast(pair, two);
+    return high ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(into, p, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(into, p, scale, false);
+}
+template <> __device__ __forceinline__ uint32_t Eight<__bf16>::bits32(uint32_t h) { return h << 16; }
+template <> __device__ __forceinline__ uint32_t Eight<_Float16>::bits32(uint32_t h) { return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)h)); }
+
+template <>
+struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+    __device__ __forceinline__ void load(const float* src, int left, int wide) {
+        if (left >= 8 && wide == 2) {
+            *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(src);
+            *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(src + 4);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? src[i] : 0.0f;
+    }
+    __device__ __forceinline__ uint32_t amax() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max_abs(m, v[i]);
+        return abs_bits(m);
+    }
+    static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float scale) {
+        i16x2 w = {0, 0};
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, scale, false);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, scale, true);
+        return __builtin_bit_cast(uint32_t, w);
+    }
+    __device__ __forceinline__ uint2 encode(float scale) const { return {encode4(v[0], v[1], v[2], v[3], scale), encode4(v[4], v[5], v[6], v[7], scale)}; }
+};
+
+// Largest magnitudes of the eight columns of eight rows, as bits of 32-bit values.
+template <typename T>
+__device__ __forceinline__ void column_amax(const Eight<T> x[8], uint32_t out[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            float m = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) m = max_abs(m, x[r].v[c]);
+            out[c] = abs_bits(m);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u16x2 m = {0, 0};
+#pragma unroll
+            for (int r = 0; r < 8; ++r) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[r].w[i] & 0x7fff7fffu));
+            out[2 * i] = Eight<T>::bits32(m[0]);
+            out[2 * i + 1] = Eight<T>::bits32(m[1]);
+        }
+    }
+}
+
+// The eight codes of column c of eight rows.
+template <typename T>
+__device__ __forceinline__ uint2 encode_column(const Eight<T> x[8], int c, float scale) {
+    if constexpr (sizeof(T) == 4) {
+        return {Eight<T>::encode4(x[0].v[c], x[1].v[c], x[2].v[c], x[3].v[c], scale), Eight<T>::encode4(x[4].v[c], x[5].v[c], x[6].v[c], x[7].v[c], scale)};
+    } else {
+        const uint32_t pick = c & 1 ? 0x07060302u : 0x05040100u;      // the high or the low halves of two words
+        Eight<T> y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y.w[i] = __builtin_amdgcn_perm(x[2 * i + 1].w[c >> 1], x[2 * i].w[c >> 1], pick);
+        return y.encode(scale);
+    }
 }
 
 }  // namespace gf

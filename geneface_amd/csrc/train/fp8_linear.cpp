@@ -1,7 +1,6 @@
 // gf_fp8_linear and gf_fp8_linear_backward: a layer's products with what they need around them, as one call each.  Host code over the entry points of
 // fp8_quantize.hip and fp8_matmul.hip; what it decides is where everything lies in the caller's two buffers.
 #include "../common.hpp"
-#include "fp8.hpp"
 #include "geneface_train_hip.h"
 
 namespace gf {

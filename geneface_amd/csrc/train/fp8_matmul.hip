@@ -37,7 +37,6 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
     const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-__device__ __forceinline__ float scale_value(int byte) { return __uint_as_float(byte ? (uint32_t)byte << 23 : 0x00400000u); }
 
 // A workgroup of 2 x 2 waves makes a tile of 64 TM x 64 TN of the product, a wave TM x TN tiles of 32 x 32.
 //
@@ -285,51 +284,68 @@ __global__ __launch_bounds__(64 * WAVES) void k_join(const float* part, uint32_t
 }
 
 // ---- a few rows ----------------------------------------------------------------------------------------------------------------------------
-// The weight's bytes bound it.  A wave takes 16 rows of the weight (one row of codes is 128 bytes a block: whole cache lines, straight into registers) and
-// every WAVES-th block; it brings the same block of x to 8 bits itself, in the registers that the matrix instruction takes it from: lane l holds row
-// l % 16 of x, values (l / 16) * 32 .. + 31 of the block, so the block's largest magnitude is two exchanges away.
-constexpr int kRowWaves = 8;
+// The weight's bytes bound it, and at the sizes it is called with, how many of them are under way at once.  A wave takes 16 rows of the weight (one row of
+// codes is 128 bytes a block: whole cache lines, straight into registers) and every 16th block, two blocks at a time, all loads before the first
+// use; 16 waves of a workgroup share the rows and add up through LDS.  A wave brings its blocks of x to 8 bits itself, in the registers that the
+// matrix instruction takes them from: lane l holds row l % 16 of x, values (l / 16) * 32 .. + 31 of the block, so the block's largest magnitude
+// is two exchanges away.
+constexpr int kRowWaves = 16, kRowBlocks = 2;
 
 template <typename T>
 __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d, const int wide) {
     __shared__ f32x4 part[kRowWaves][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    const uint64_t n0 = (uint64_t)blockIdx.x * 16, blocks = (d.k + 127) / 128;
+    const uint64_t n0 = (uint64_t)blockIdx.x * 16;
+    const uint32_t blocks = (uint32_t)((d.k + 127) / 128);
     const uint64_t row = min(n0 + r, d.n - 1);
     const uint8_t* w = d.codes + row * blocks * 128 + q * 32;
     const uint8_t* ws = d.scales + (row >> 7) * blocks;
     const T* x = (const T*)d.x + min((uint64_t)r, d.m - 1) * d.ldx;
+    const bool there = (uint32_t)r < d.m;
     f32x4 acc = {0, 0, 0, 0};
-    for (uint64_t b = wave; b < blocks; b += kRowWaves) {
-        const i32x4 lo = *reinterpret_cast<const i32x4*>(w + b * 128), hi = *reinterpret_cast<const i32x4*>(w + b * 128 + 16);
-        const int sw = ws[b];
-        float v[32];
-        const uint64_t k0 = b * 128 + q * 32;
+    for (uint32_t b0 = wave; b0 < blocks; b0 += kRowWaves * kRowBlocks) {
+        i32x4 lo[kRowBlocks], hi[kRowBlocks];
+        int sw[kRowBlocks];
+        Eight<T> v[kRowBlocks][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint64_t k = k0 + 4 * i;
-            const int left = (uint32_t)r < d.m && k < d.k ? (int)min((uint64_t)4, d.k - k) : 0;
-            load4_of(x + (left ? k : 0), left, wide, v + 4 * i);
+        for (int u = 0; u < kRowBlocks; ++u) {      // behind the last block: that one again, with an x of zeros
+            const uint64_t b = min(b0 + u * kRowWaves, blocks - 1);
+            lo[u] = *reinterpret_cast<const i32x4*>(w + b * 128);
+            hi[u] = *reinterpret_cast<const i32x4*>(w + b * 128 + 16);
+            sw[u] = ws[b];
         }
-        uint32_t a = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) a = max(a, abs_bits(v[i]));
-        a = max(a, (uint32_t)__shfl_xor((int)a, 16));
-        a = max(a, (uint32_t)__shfl_xor((int)a, 32));
-        const uint32_t sx = scale_byte(a);
-        const float inv = scale_inverse(sx);
-        i32x8 fx;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) fx[i] = (int)encode4(v + 4 * i, inv);
-        if constexpr (sizeof(T) == 4) {      // a 32-bit result: see EXACT above
+        for (int u = 0; u < kRowBlocks; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const i32x4 part = i < 2 ? lo : hi;
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(part[2 * (i & 1)], part[2 * (i & 1) + 1], scale_value(sw)),
-                                                              widen8(fx[2 * i], fx[2 * i + 1], scale_value((int)sx)), acc, 0, 0, 0);
+                const uint64_t k = (uint64_t)(b0 + u * kRowWaves) * 128 + q * 32 + 8 * i;
+                const int left = there && k < d.k ? (int)min((uint64_t)8, d.k - k) : 0;
+                v[u][i].load(x + (left ? k : 0), left, wide);
             }
-        } else {
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), fx, acc, 0, 0, 0, sw, 0, (int)sx);
+#pragma unroll
+        for (int u = 0; u < kRowBlocks; ++u) {
+            uint32_t a = max(max(v[u][0].amax(), v[u][1].amax()), max(v[u][2].amax(), v[u][3].amax()));
+            a = max(a, (uint32_t)__shfl_xor((int)a, 16));
+            a = max(a, (uint32_t)__shfl_xor((int)a, 32));
+            const uint32_t sx = scale_byte(a);
+            const float scale = scale_value(sx);
+            i32x8 fx;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint2 c = coded(v[u][i].encode(scale), sx);
+                fx[2 * i] = (int)c.x;
+                fx[2 * i + 1] = (int)c.y;
+            }
+            if constexpr (sizeof(T) == 4) {      // a 32-bit result: see EXACT above
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const i32x4 part = i < 2 ? lo[u] : hi[u];
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(part[2 * (i & 1)], part[2 * (i & 1) + 1], scale_value(sw[u])),
+                                                                  widen8(fx[2 * i], fx[2 * i + 1], scale), acc, 0, 0, 0);
+                }
+            } else {
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(lo[u], hi[u], 0, 1, 2, 3, 4, 5, 6, 7), fx, acc, 0, 0, 0, sw[u], 0, (int)sx);
+            }
         }
     }
     part[wave][lane] = acc;
@@ -438,10 +454,12 @@ GF_EXPORT int gf_fp8_rows(const gf_fp8_rows_t* d, void* stream) {
     if (d->m > 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: at most 16 rows, got %llu", (unsigned long long)d->m);
     if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: unknown dtype %u", d->dtype);
     if (d->k == 0 || d->ldx < d->k) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: ldx < k, or k = 0");
+    if (d->k >> 31) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: matrix too large");
     if ((uintptr_t)d->codes % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: codes must start at a multiple of 16 bytes");
     if ((d->n + 15) / 16 >> 31) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: matrix too large");
     const uint64_t size = d->dtype == F32 ? 4 : 2;
-    const int wide = ((uintptr_t)d->x | d->ldx * size) % (4 * size) == 0;
+    const uint64_t at = (uintptr_t)d->x | (d->m > 1 ? d->ldx * size : 0);
+    const int wide = at % 16 == 0 ? 2 : size == 2 && at % 8 == 0 ? 1 : 0;
     const uint32_t grid = (uint32_t)((d->n + 15) / 16);
     const hipStream_t s = gf_stream(stream);
     if (d->dtype == F32) k_rows<float><<<grid, 64 * kRowWaves, 0, s>>>(*d, wide);
