@@ -50,8 +50,12 @@ TRAIN_DIR = os.path.join(HERE, "train")
 TRAIN_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option"]
 
 
+HOST_SOURCE = os.path.join(TRAIN_DIR, "host.cpp")      # the one file that includes torch's headers: a Python module of its own
+HOST_OUT = os.path.join(HERE, "_train_host.so")
+
+
 def train_sources():
-    return sorted(glob.glob(os.path.join(TRAIN_DIR, "*.hip")) + glob.glob(os.path.join(TRAIN_DIR, "*.cpp")))
+    return sorted({*glob.glob(os.path.join(TRAIN_DIR, "*.hip")), *glob.glob(os.path.join(TRAIN_DIR, "*.cpp"))} - {HOST_SOURCE})
 
 
 def train_headers():
@@ -93,6 +97,25 @@ def _compile(src, force, extra=(), obj_dir=OBJ_DIR, drop=()):
     return obj, True
 
 
+def build_host(force: bool = False) -> str:
+    """_train_host.so: the operators' argument checks and calls in C++ against this interpreter's torch (lib.host() loads it)."""
+    newest = max(os.path.getmtime(p) for p in [HOST_SOURCE, __file__, train_headers()[-1]])
+    if not force and os.path.exists(HOST_OUT) and os.path.getmtime(HOST_OUT) >= newest:
+        return HOST_OUT
+    import sysconfig
+    import torch
+    home = os.path.join(os.path.dirname(torch.__file__))
+    inc = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+           "/opt/rocm/include", os.path.join(HERE, "..", "..", "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_train_host", *[f"-I{i}" for i in inc], HOST_SOURCE,
+           "-o", HOST_OUT, f"-L{os.path.join(home, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {HOST_SOURCE}:\n{r.stdout}\n{r.stderr}")
+    return HOST_OUT
+
+
 def build(force: bool = False, verbose: bool = False, trace: bool = False, variant: str = None, defines=(), drop_flags=()) -> str:
     """trace=True builds the instrumented variant (-DGF_TRACE: per-round s_memtime timeline of the head kernel, read by
     tools/trace_head.py) into libgeneface_hip_trace.so; the product library never contains the instrumentation.
@@ -106,7 +129,10 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, varia
     extra = (("-DGF_TRACE",) if trace else ()) + tuple(defines)
     os.makedirs(os.path.join(obj_dir, "train"), exist_ok=True)
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        host = ex.submit(build_host, force) if not tag else None
         results = list(ex.map(lambda s: _compile(s, force, extra, obj_dir, tuple(drop_flags)), [*sources(), *train_sources()]))
+        if host is not None:
+            host.result()
     objs = [o for o, _ in results]
     if force or any(ch for _, ch in results) or not os.path.exists(out):
         cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *objs, "-o", out, "-lz", "-lpthread"]   # zlib: the PNG frame writer (png_writer.cpp)

@@ -17,7 +17,7 @@ import ctypes as C
 
 import torch
 
-from .lib import check, current_stream, lib
+from .lib import check, current_stream, host, lib
 from .optim import DTYPES
 
 BLOCK = 128
@@ -54,16 +54,6 @@ def _matrix(x):
     return m if m.stride(1) == 1 and m.stride(0) >= m.shape[1] else m.contiguous()
 
 
-def _check_type(name, t):
-    if t.dtype not in DTYPES:
-        raise RuntimeError(f"fp8: {name} must be float32, bfloat16 or float16, got {t.dtype}")
-
-
-def _check_device(name, t):
-    if t.device.type != "cuda":
-        raise RuntimeError(f"fp8: {name} must be a CUDA tensor")
-
-
 def _quantize(m, rows, cols, tiles=False):
     """(row codes, row scales, column codes, column scales) of m [R, C]; with `tiles` one tensor of scales for both.  What is not wanted is None."""
     R, Cn = m.shape
@@ -85,6 +75,8 @@ class Fp8Weight:
 
     values: float8_e4m3fn [N, up(K)], up(K) the multiple of 128 that holds K, zeros behind K; scales: float8_e8m0fnu [ceil(N / 128), ceil(K / 128)];
     in_features: K."""
+
+    __slots__ = ("values", "scales", "in_features", "out_features")
 
     def __init__(self, values, scales, in_features):
         if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float8_e8m0fnu:
@@ -116,10 +108,12 @@ class Fp8Weight:
 @torch.no_grad()
 def quantize_weight(weight):
     """Fp8Weight of weight [N, K] (float32, bfloat16 or float16)."""
-    _check_type("the weight", weight)
+    if weight.dtype not in DTYPES:
+        raise RuntimeError(f"fp8: the weight must be float32, bfloat16 or float16, got {weight.dtype}")
     if weight.dim() != 2:
         raise RuntimeError(f"fp8: the weight must be a matrix, got {tuple(weight.shape)}")
-    _check_device("the weight", weight)
+    if not weight.is_cuda:
+        raise RuntimeError("fp8: the weight must be a CUDA tensor")
     N, K = weight.shape
     with torch.cuda.device(weight.device):
         if N and K:
@@ -129,96 +123,11 @@ def quantize_weight(weight):
     return Fp8Weight(codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu), K)
 
 
-def _forward(x, w, packed, keep_w, keep_x):
-    """(y, what the backward pass needs, its workspace's bytes) of x [M, K] and w [N, K], on x's device."""
-    dev = x.device
-    M, K = x.shape
-    N = w.out_features if packed else w.shape[0]
-    d = GfFp8Linear(x.data_ptr(), x.stride(0) if M > 1 else K, m=M, n=N, k=K, dtype=DTYPES[x.dtype], keep_w=keep_w, keep_x=keep_x)
-    if packed:
-        d.codes, d.scales = w.values.data_ptr(), w.scales.data_ptr()
-    else:
-        d.w, d.ldw, d.w_dtype = w.data_ptr(), w.stride(0) if N > 1 else K, DTYPES[w.dtype]
-    L = lib()
-    check(L.gf_fp8_linear_plan(C.byref(d)))
-    y = torch.empty(M, N, dtype=x.dtype, device=dev)
-    saved = torch.empty(d.saved_bytes, dtype=torch.uint8, device=dev) if d.saved_bytes else None
-    work = torch.empty(d.workspace_bytes, dtype=torch.uint8, device=dev) if d.workspace_bytes else None
-    d.y, d.saved, d.workspace = y.data_ptr(), None if saved is None else saved.data_ptr(), None if work is None else work.data_ptr()
-    check(L.gf_fp8_linear(C.byref(d), current_stream(dev)))
-    return y, saved, d.backward_bytes
-
-
-class _on:
-    """torch.cuda.device(dev), entered only where it is not the current device already."""
-    def __init__(self, dev):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight):
-        keep_w, keep_x = ctx.needs_input_grad
-        with _on(x.device):
-            y, saved, ctx.backward_bytes = _forward(_matrix(x), _matrix(weight), False, keep_w, keep_x)
-        ctx.save_for_backward(saved)      # w by columns and x by columns, in 8 bits: neither tensor itself
-        ctx.sizes, ctx.dtypes, ctx.keep = (*x.shape, weight.shape[0]), (x.dtype, weight.dtype), (keep_w, keep_x)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        saved, = ctx.saved_tensors
-        (M, K, N), (tx, tw), (keep_w, keep_x) = ctx.sizes, ctx.dtypes, ctx.keep
-        want_x, want_w = ctx.needs_input_grad
-        dev, dy = dy.device, _matrix(dy)
-        with _on(dev):
-            dx = torch.empty(M, K, dtype=tx, device=dev) if want_x else None
-            dw = torch.empty(N, K, dtype=tw, device=dev) if want_w else None
-            work = torch.empty(ctx.backward_bytes, dtype=torch.uint8, device=dev)
-            d = GfFp8LinearBackward(dy.data_ptr(), dy.stride(0) if M > 1 else N, saved.data_ptr(), M, N, K, dx.data_ptr() if want_x else None,
-                                    dw.data_ptr() if want_w else None, work.data_ptr(), DTYPES[tx], DTYPES[tw], keep_w, keep_x)
-            check(lib().gf_fp8_linear_backward(C.byref(d), current_stream(dev)))
-        return dx, dw
-
-
 def linear(x, weight):
     """x [..., K] times a weight's transpose, [..., N] in x's type (under autocast: in its type), both brought to 8 bits in blocks of 128.
 
     weight: a tensor [N, K], quantised in the call, with gradients to x and to the weight; or an Fp8Weight, without gradients.  x, weight: float32,
     bfloat16 or float16, each its own; the gradients have their input's type."""
-    packed = isinstance(weight, Fp8Weight)
-    if not packed:
-        _check_type("the weight", weight)
-        if weight.dim() != 2:
-            raise RuntimeError(f"fp8: the weight must be a matrix, got {tuple(weight.shape)}")
-    K = weight.in_features if packed else weight.shape[1]
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise RuntimeError(f"fp8: x of shape {tuple(x.shape)} does not fit a weight of {K} input features")
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
-        x = x.to(torch.get_autocast_dtype("cuda"))
-    _check_type("x", x)
-    _check_device("x", x)
-    if x.device != weight.device:
-        raise RuntimeError(f"fp8: x is on {x.device}, the weight on {weight.device}")
-    if packed:
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("fp8: an Fp8Weight has no backward pass: give the weight itself, or call under no_grad")
-        N = weight.out_features
-        if not (x.numel() and N):
-            return torch.zeros(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-        with _on(x.device):
-            y = _forward(_matrix(x), weight, True, False, False)[0]
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
-    if not (x.numel() and weight.numel()):      # nothing to add up; differentiable
-        return x @ weight.t().to(x.dtype)
-    y = _Linear.apply(x.reshape(-1, K), weight)      # (a view made inside the node could not be written in place, as MLP's ReLU does)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
+    if isinstance(weight, Fp8Weight):
+        return host().linear_packed(x, weight.values, weight.scales, weight.in_features)
+    return host().linear(x, weight)

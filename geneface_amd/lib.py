@@ -81,6 +81,29 @@ def lib():
     return _lib
 
 
+_host = None
+_HOST_CALLS = ("gf_adamw_step", "gf_grad_norm_workspace_bytes", "gf_grad_norm", "gf_fp8_linear_plan", "gf_fp8_linear", "gf_fp8_linear_backward", "gf_last_error")
+
+
+def host():
+    """The C++ host half of the training operators (csrc/train/host.cpp), bound to the loaded library's functions."""
+    global _host
+    if _host is None:
+        L = lib()
+        with _lock:
+            if _host is None:
+                from .csrc import build as _b
+                if not os.path.exists(_b.HOST_OUT):
+                    _b.build_host()
+                try:
+                    from .csrc import _train_host
+                except ImportError as e:
+                    raise RuntimeError(f"geneface_amd: cannot load {_b.HOST_OUT}: {e}. Run `python -c 'import __graft_entry__ as g; g.build()'`.") from e
+                _train_host.bind([C.cast(getattr(L, n), C.c_void_p).value for n in _HOST_CALLS])
+                _host = _train_host
+    return _host
+
+
 def check(rc: int):
     if rc != 0:
         raise RuntimeError(lib().gf_last_error().decode())

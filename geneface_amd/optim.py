@@ -17,7 +17,7 @@ import math
 
 import torch
 
-from .lib import check, current_stream, lib
+from .lib import host
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 BLOCK = 128
@@ -37,54 +37,12 @@ class GfGradNorm(C.Structure):
     _fields_ = [("tensors_host", _vp), ("count", C.c_uint32), ("_pad", C.c_uint32)] + [(n, _vp) for n in ("grad_scale", "norm_out", "workspace")]
 
 
-# a step asks these of hundreds of tensors: mapped over whole lists they cost a tenth of a microsecond each
-_ptr, _numel, _contiguous, _device_index = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
-_dtype, _layout = torch.Tensor.dtype.__get__, torch.Tensor.layout.__get__
-
-
-def _same_device(name, tensors, device):
-    if device.type != "cuda":
-        raise RuntimeError(f"{name} must be CUDA tensors")
-    if {*map(_device_index, tensors)} != {device.index}:
-        raise RuntimeError(f"{name} must all be on {device}")
-
-
-def _scalar(name, t, device):
-    """Address of one float32 on the device, or None."""
-    if t is None:
-        return None
-    if not torch.is_tensor(t) or t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
-        raise RuntimeError(f"{name} must be one float32 value on {device}")
-    return t.data_ptr()
-
-
 def grad_norm(grads, grad_scale=None):
     """sqrt(sum of the squares of all `grads`) / grad_scale as a float32 tensor without dimensions, added up in 64 bits in a fixed order.
 
     grads: tensors of float32, bfloat16 or float16 on one device (None entries are left out).  grad_scale: one float32 on that device, the
     factor the gradients carry (GradScaler's scale).  Infinities and NaN among the gradients give an infinite norm or NaN."""
-    grads = [g for g in grads if g is not None]
-    if not grads:
-        raise RuntimeError("grad_norm: no gradients")
-    if {*map(_layout, grads)} != {torch.strided}:
-        raise RuntimeError("grad_norm: sparse gradients are not supported")
-    dev = grads[0].device
-    dtypes = [DTYPES.get(d) for d in map(_dtype, grads)]
-    if None in dtypes:
-        raise RuntimeError("grad_norm: gradients must be float32, bfloat16 or float16")
-    _same_device("grad_norm: the gradients", grads, dev)
-    with torch.cuda.device(dev):
-        if not all(map(_contiguous, grads)):
-            grads = [g.contiguous() for g in grads]
-        scale = _scalar("grad_scale", grad_scale, dev)
-        L, n = lib(), len(grads)
-        out = torch.empty((), dtype=torch.float32, device=dev)
-        workspace = torch.empty(L.gf_grad_norm_workspace_bytes(n) // 8, dtype=torch.float64, device=dev)
-        table = (C.c_uint64 * (3 * n))()
-        table[0::3], table[1::3], table[2::3] = list(map(_ptr, grads)), list(map(_numel, grads)), dtypes
-        d = GfGradNorm(C.addressof(table), n, 0, scale, out.data_ptr(), workspace.data_ptr())
-        check(L.gf_grad_norm(C.byref(d), current_stream(dev)))
-    return out
+    return host().grad_norm([g for g in grads if g is not None], grad_scale)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, exp_avg_scales=None,
@@ -98,78 +56,18 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     lr: a number, or one float32 on the device.  grad_scale: the factor that the gradients carry.  found_inf: where it is not 0 nothing is
     changed, the step counts included.  grad_norm, max_norm: gradients are multiplied by min(1, max_norm / (grad_norm + 1e-6)); both or neither.
     grad_scale, found_inf, grad_norm: one float32 on the device each.  Gradients are only read: they keep their factor."""
-    eight = exp_avg_scales is not None or exp_avg_sq_scales is not None
-    lists = [params, grads, exp_avgs, exp_avg_sqs, steps] + ([exp_avg_scales, exp_avg_sq_scales] if eight else [])
-    if any(v is None for v in lists):
+    if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
         raise RuntimeError("adamw_step: exp_avg_scales and exp_avg_sq_scales must both be given for 8-bit moments")
-    lists = [list(v) for v in lists]
-    params, grads, exp_avgs, exp_avg_sqs, steps = lists[:5]
-    n = len(params)
-    if any(len(v) != n for v in lists):
-        raise RuntimeError(f"adamw_step: lists of unlike lengths {[len(v) for v in lists]}")
     beta1, beta2 = map(float, betas)
     if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
         raise ValueError(f"adamw_step: betas must be in [0, 1), got {betas}")
     if (grad_norm is None) != (max_norm is None):
         raise RuntimeError("adamw_step: grad_norm and max_norm go together")
-    if not n:
-        return
-    dev = params[0].device
-    sizes = list(map(_numel, params))
-    if {*map(_layout, grads)} != {torch.strided}:
-        raise RuntimeError("adamw_step: sparse gradients are not supported")
-    types = list(map(_dtype, params))
-    if list(map(_dtype, grads)) != types:
-        raise RuntimeError("adamw_step: a gradient must have its parameter's dtype")
-    kinds = set(types)
-    if not kinds <= DTYPES.keys():
-        raise RuntimeError("adamw_step: parameters must be float32, bfloat16 or float16")
-    if any(list(map(_numel, v)) != sizes for v in lists[1:4]):
-        raise RuntimeError("adamw_step: gradients and moments must have their parameter's size")
-    state = torch.float8_e4m3fn if eight else torch.float32
-    if {*map(_dtype, exp_avgs), *map(_dtype, exp_avg_sqs)} != {state}:
-        raise RuntimeError(f"adamw_step: moments must be {state} {'with' if eight else 'without'} scales")
-    if {*map(_dtype, steps)} != {torch.float32} or {*map(_numel, steps)} != {1}:
-        raise RuntimeError("adamw_step: each step must be one float32 value")
-    if eight:
-        blocks = [-(-k // BLOCK) for k in sizes]
-        for v in lists[5:]:
-            if {*map(_dtype, v)} != {torch.float32} or list(map(_numel, v)) != blocks:
-                raise RuntimeError("adamw_step: scales must be float32 with one value for each 128 of the parameter")
-    _same_device("adamw_step: all tensors", [t for v in lists for t in v], dev)
-    if not all(map(_contiguous, grads)):
-        with torch.cuda.device(dev):
-            grads = lists[1] = [g.contiguous() for g in grads]
-    if not all(map(_contiguous, [t for v in lists for t in v])):
-        raise RuntimeError("adamw_step: parameters and their state must be contiguous tensors")
-    pointers = [list(map(_ptr, v)) for v in lists]
-    for k, v in enumerate(pointers):
-        if k != 1 and len({*v}) != n and (k == 4 or len({a for a, size in zip(v, sizes) if size}) != n - sizes.count(0)):      # (empty tensors have no address)
-            raise RuntimeError("adamw_step: the same tensor is given twice")
     lr_device = None
-    if torch.is_tensor(lr):
-        if lr.is_cuda:
-            lr, lr_device = 0.0, _scalar("lr", lr, dev)
-        else:
-            lr = float(lr)
-    scalars = [_scalar(k, t, dev) for k, t in (("grad_scale", grad_scale), ("found_inf", found_inf), ("grad_norm", grad_norm))]
-    L = lib()
-    with torch.cuda.device(dev):
-        for kind in sorted(kinds, key=DTYPES.get):
-            pick = pointers + [sizes]
-            if len(kinds) > 1:
-                at = [i for i in range(n) if types[i] == kind]
-                pick = [[v[i] for i in at] for v in pick]
-            p, g, m, v, step = pick[:5]
-            count = len(p)
-            table = (C.c_uint64 * (8 * count))()
-            table[0::8], table[1::8], table[2::8], table[3::8], table[6::8], table[7::8] = p, g, m, v, step, pick[-1]
-            if eight:
-                table[4::8], table[5::8] = pick[5], pick[6]
-            d = GfAdamw(C.addressof(table), count, DTYPES[kind], 8 if eight else 32, 0, float(lr), beta1, beta2, float(eps), float(weight_decay),
-                        math.inf if max_norm is None else float(max_norm), lr_device, *scalars)
-            check(L.gf_adamw_step(C.byref(d), current_stream(dev)))
-    torch.autograd.graph.increment_version([t for k, v in enumerate(lists) if k != 1 for t in v])      # written through raw pointers
+    if torch.is_tensor(lr) and lr.is_cuda:
+        lr, lr_device = 0.0, lr
+    host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, float(lr), lr_device, beta1, beta2, float(eps), float(weight_decay), exp_avg_scales,
+                      exp_avg_sq_scales, grad_scale, found_inf, grad_norm, math.inf if max_norm is None else float(max_norm))
 
 
 class AdamW(torch.optim.Optimizer):
