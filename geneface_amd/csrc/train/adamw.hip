@@ -12,7 +12,6 @@ namespace gf {
 
 constexpr int kThreads = 256;
 constexpr int kTensors = 56;              // per launch: 56 x 64 bytes + first workgroups + scalars < 4096
-constexpr uint64_t kNarrow = 1ull << 63;  // flag in n: an address of this tensor is no multiple of four values
 
 struct AdamwArgs {
     gf_adamw_tensor_t t[kTensors];
@@ -76,17 +75,17 @@ __device__ __forceinline__ uint32_t tensor_of(const AdamwArgs& a, uint32_t block
 
 // 32-bit moments: four consecutive values a thread.
 template <typename T>
-__device__ __forceinline__ void step32(const gf_adamw_tensor_t& t, const Hyper& h, uint64_t begin, uint64_t end, bool wide) {
+__device__ __forceinline__ void step32(const gf_adamw_tensor_t& t, const Hyper& h, uint64_t begin, uint64_t end) {
     T* p = (T*)t.p;
     const T* g = (const T*)t.g;
     float *m = (float*)t.m, *v = (float*)t.v;
     for (uint64_t i = begin + threadIdx.x * 4; i < end; i += kThreads * 4) {
         const int left = (int)min((uint64_t)4, end - i);
         float fp[4], fg[4], fm[4], fv[4];
-        load4_of(g + i, left, wide, fg);
-        load4_of(m + i, left, wide, fm);
-        load4_of(v + i, left, wide, fv);
-        load4_of(p + i, left, wide, fp);
+        load4_of(g + i, left, fg);
+        load4_of(m + i, left, fm);
+        load4_of(v + i, left, fv);
+        load4_of(p + i, left, fp);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float x = fg[k] * h.grad;
@@ -94,9 +93,9 @@ __device__ __forceinline__ void step32(const gf_adamw_tensor_t& t, const Hyper& 
             fv[k] = moment2(h, fv[k], x);
             fp[k] = updated(h, fp[k], fm[k], sqrtf(fv[k]));
         }
-        store4_of(m + i, left, wide, fm);
-        store4_of(v + i, left, wide, fv);
-        store4_of(p + i, left, wide, fp);
+        store4_of(m + i, left, fm);
+        store4_of(v + i, left, fv);
+        store4_of(p + i, left, fp);
     }
 }
 
@@ -124,21 +123,22 @@ __device__ __forceinline__ void decode4(uint32_t w, float scale, float out[4]) {
     out[0] = lo[0] * scale; out[1] = lo[1] * scale; out[2] = hi[0] * scale; out[3] = hi[1] * scale;
 }
 
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int left, bool wide) {
-    if (wide && left >= 4) return *reinterpret_cast<const uint32_t*>(src);
+typedef uint32_t codes4 __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int left) {
+    if (left >= 4) return *reinterpret_cast<const codes4*>(src);
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (i < left) w |= (uint32_t)src[i] << (8 * i);
     return w;
 }
-__device__ __forceinline__ void store_codes(uint8_t* dst, uint32_t w, int left, bool wide) {
-    if (wide && left >= 4) { *reinterpret_cast<uint32_t*>(dst) = w; return; }
+__device__ __forceinline__ void store_codes(uint8_t* dst, uint32_t w, int left) {
+    if (left >= 4) { *reinterpret_cast<codes4*>(dst) = w; return; }
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (i < left) dst[i] = (uint8_t)(w >> (8 * i));
 }
 
 template <typename T>
-__device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h, uint64_t begin, uint64_t end, bool wide, uint32_t word) {
+__device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h, uint64_t begin, uint64_t end, uint32_t word) {
     T* p = (T*)t.p;
     const T* g = (const T*)t.g;
     uint8_t *m = (uint8_t*)t.m, *v = (uint8_t*)t.v;
@@ -154,10 +154,10 @@ __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h
             const uint64_t i = i0 + 64 * q;
             left[q] = i < end ? (int)min((uint64_t)4, end - i) : 0;
             const uint64_t at = left[q] ? i : begin;
-            load4_of(g + at, left[q], wide, fg + 4 * q);
-            load4_of(p + at, left[q], wide, fp + 4 * q);
-            decode4(load_codes(m + at, left[q], wide), ms, fm + 4 * q);
-            decode4(load_codes(v + at, left[q], wide), vs, fr + 4 * q);
+            load4_of(g + at, left[q], fg + 4 * q);
+            load4_of(p + at, left[q], fp + 4 * q);
+            decode4(load_codes(m + at, left[q]), ms, fm + 4 * q);
+            decode4(load_codes(v + at, left[q]), vs, fr + 4 * q);
         }
         float am = 0, ar = 0;
 #pragma unroll
@@ -187,9 +187,9 @@ __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h
             const uint32_t wm = encode_dithered4(ym, seed), wr = encode_dithered4(yr, seed ^ 0x80000000u);
             if (left[q]) {
                 const uint64_t i = i0 + 64 * q;
-                store_codes(m + i, wm, left[q], wide);
-                store_codes(v + i, wr, left[q], wide);
-                store4_of(p + i, left[q], wide, fp + 4 * q);
+                store_codes(m + i, wm, left[q]);
+                store_codes(v + i, wr, left[q]);
+                store4_of(p + i, left[q], fp + 4 * q);
             }
         }
         if (lane16 == 0) { t.m_scale[b] = a_m / 448.0f; t.v_scale[b] = a_r / 448.0f; }
@@ -201,13 +201,11 @@ __global__ __launch_bounds__(kThreads) void k_adamw(const AdamwArgs a) {
     if (a.found_inf && *a.found_inf != 0.0f) return;
     const uint32_t at = tensor_of(a, blockIdx.x);
     const gf_adamw_tensor_t t = a.t[at];
-    const uint64_t n = t.n & ~kNarrow, begin = (uint64_t)(blockIdx.x - a.first[at]) * a.chunk;
-    const bool wide = !(t.n & kNarrow);
+    const uint64_t begin = (uint64_t)(blockIdx.x - a.first[at]) * a.chunk, end = min(t.n, begin + a.chunk);
     const float now = *t.step + 1.0f;
     const Hyper h = hyper_of(a, now);
-    const uint64_t end = min(n, begin + a.chunk);
-    if constexpr (BITS == 32) step32<T>(t, h, begin, end, wide);
-    else step8<T>(t, h, begin, end, wide, (uint32_t)now * kDitherStep);
+    if constexpr (BITS == 32) step32<T>(t, h, begin, end);
+    else step8<T>(t, h, begin, end, (uint32_t)now * kDitherStep);
     if (a.count_steps) {
         __syncthreads();                  // the tensor's only workgroup: every thread has read the count
         if (threadIdx.x == 0) *t.step = now;
@@ -250,20 +248,24 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
 
 // Squares are added up in 64 bits: a 32-bit square leaves the type's range at 1e19 and at 1e-23, and the sum is one over all values of a model.
 template <typename T>
-__device__ __forceinline__ double squares(const T* g, uint64_t begin, uint64_t end, bool wide) {
+__device__ __forceinline__ double squares(const T* g, uint64_t begin, uint64_t end) {
     double s[4] = {0, 0, 0, 0};
-    for (uint64_t i = begin + threadIdx.x * 4; i < end; i += kThreads * 16) {
-        float f[4][4];
+    uint64_t i = begin + threadIdx.x * 4;
+    constexpr int U = 8;                  // loads under way
+    for (; i + (U - 1) * kThreads * 4 + 4 <= end; i += U * kThreads * 4) {
+        float f[U][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint64_t j = i + q * kThreads * 4;
-            const int left = j < end ? (int)min((uint64_t)4, end - j) : 0;
-            load4_of(g + (left ? j : begin), left, wide, f[q]);
-        }
+        for (int q = 0; q < U; ++q) load4(g + i + q * kThreads * 4, f[q]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < U; ++q)
 #pragma unroll
             for (int k = 0; k < 4; ++k) s[k] = fma((double)f[q][k], (double)f[q][k], s[k]);
+    }
+    for (; i < end; i += kThreads * 4) {
+        float f[4];
+        load4_of(g + i, (int)min((uint64_t)4, end - i), f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] = fma((double)f[k], (double)f[k], s[k]);
     }
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
@@ -276,12 +278,11 @@ __global__ __launch_bounds__(kThreads) void k_norm(const NormArgs a) {
         at += (uint32_t)__popcll(__ballot(r + lane < kNormTensors && a.first[r + lane < kNormTensors ? r + lane : 0] <= blockIdx.x));
     at = __builtin_amdgcn_readfirstlane(at) - 1;
     const gf_norm_tensor_t t = a.t[at];
-    const uint64_t n = t.n & ~kNarrow, begin = (blockIdx.x - a.first[at]) * a.chunk, end = min(n, begin + a.chunk);
-    const bool wide = !(t.n & kNarrow);
+    const uint64_t begin = (blockIdx.x - a.first[at]) * a.chunk, end = min(t.n, begin + a.chunk);
     double s;
-    if (t.dtype == F32) s = squares((const float*)t.g, begin, end, wide);
-    else if (t.dtype == BF16) s = squares((const __bf16*)t.g, begin, end, wide);
-    else s = squares((const _Float16*)t.g, begin, end, wide);
+    if (t.dtype == F32) s = squares((const float*)t.g, begin, end);
+    else if (t.dtype == BF16) s = squares((const __bf16*)t.g, begin, end);
+    else s = squares((const _Float16*)t.g, begin, end);
     s = block_sum(s, lds);
     if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
 }
@@ -293,9 +294,6 @@ __global__ __launch_bounds__(1024) void k_norm_finish(const double* sums, uint32
     s = block_sum(s, lds);
     if (threadIdx.x == 0) *out = (float)(sqrt(s) / (grad_scale ? (double)*grad_scale : 1.0));
 }
-
-static uint32_t elem_bytes(uint32_t dtype) { return dtype == F32 ? 4 : 2; }
-static bool off(const void* p, uint32_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 
 }  // namespace gf
 
@@ -329,14 +327,12 @@ GF_EXPORT int gf_adamw_step(const gf_adamw_t* d, void* stream) {
     a.chunk = chunk;
     a.count_steps = most <= chunk;
     a.lr_device = d->lr_device; a.grad_scale = d->grad_scale; a.found_inf = d->found_inf; a.grad_norm = d->grad_norm;
-    const uint32_t eb = elem_bytes(d->dtype), sb = d->state_bits / 8;
     const hipStream_t s = gf_stream(stream);
     for (uint32_t i = 0; i < d->count;) {
         uint32_t k = 0, blocks = 0;
         for (; i < d->count && k < kTensors; ++i, ++k) {
-            gf_adamw_tensor_t t = d->tensors_host[i];
+            const gf_adamw_tensor_t& t = d->tensors_host[i];
             const uint32_t need = t.n ? (uint32_t)((t.n + chunk - 1) / chunk) : 1;       // an empty tensor's step is counted too
-            if (off(t.p, 4 * eb) || off(t.g, 4 * eb) || off(t.m, 4 * sb) || off(t.v, 4 * sb)) t.n |= kNarrow;
             a.t[k] = t;
             a.first[k] = blocks;
             blocks += need;
@@ -378,10 +374,9 @@ GF_EXPORT int gf_grad_norm(const gf_grad_norm_t* d, void* stream) {
         int k = 0;
         uint32_t blocks = 0;
         for (; i < d->count && k < kNormTensors; ++i) {
-            gf_norm_tensor_t t = d->tensors_host[i];
+            const gf_norm_tensor_t& t = d->tensors_host[i];
             if (!t.n) continue;
             const uint32_t need = (uint32_t)((t.n + a.chunk - 1) / a.chunk);
-            if (off(t.g, 4 * elem_bytes(t.dtype))) t.n |= kNarrow;
             a.t[k] = t;
             a.first[k++] = blocks;
             blocks += need;

@@ -7,12 +7,12 @@ namespace gf {
 
 enum { F32 = 0, BF16 = 1, F16 = 2 };
 
+// Four consecutive values at any address that their type allows: the memory pipeline takes 16- and 8-byte accesses at any of them.
 template <typename T> struct Vec4;
-template <> struct Vec4<float> { typedef float type __attribute__((ext_vector_type(4))); };
-template <> struct Vec4<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
-template <> struct Vec4<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
+template <> struct Vec4<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Vec4<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Vec4<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
 
-// four values from / to an address that is a multiple of their size
 template <typename T>
 __device__ __forceinline__ void load4(const T* src, float out[4]) {
     const typename Vec4<T>::type v = *reinterpret_cast<const typename Vec4<T>::type*>(src);
@@ -27,16 +27,16 @@ __device__ __forceinline__ void store4(T* dst, const float in[4]) {
     *reinterpret_cast<typename Vec4<T>::type*>(dst) = v;
 }
 
-// four values of which the first `left` exist (0 for the others); `wide`: the address is a multiple of four values
+// four values of which the first `left` exist (0 for the others)
 template <typename T>
-__device__ __forceinline__ void load4_of(const T* src, int left, bool wide, float out[4]) {
-    if (wide && left >= 4) { load4(src, out); return; }
+__device__ __forceinline__ void load4_of(const T* src, int left, float out[4]) {
+    if (left >= 4) { load4(src, out); return; }
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = i < left ? (float)src[i] : 0.0f;
 }
 template <typename T>
-__device__ __forceinline__ void store4_of(T* dst, int left, bool wide, const float in[4]) {
-    if (wide && left >= 4) { store4(dst, in); return; }
+__device__ __forceinline__ void store4_of(T* dst, int left, const float in[4]) {
+    if (left >= 4) { store4(dst, in); return; }
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (i < left) dst[i] = (T)in[i];
 }

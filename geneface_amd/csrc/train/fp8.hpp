@@ -38,14 +38,9 @@ struct Eight {      // 16-bit types
     uint32_t w[4];
     typedef T pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ i16x2 encode2(i16x2 into, uint32_t two, float scale, bool high);
-    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
-    __device__ __forceinline__ void load(const T* src, int left, int wide) {      // wide: 2: a multiple of 16 bytes, 1: of 8, 0: of 2
-        if (left >= 8 && wide == 2) { *reinterpret_cast<i32x4*>(w) = *reinterpret_cast<const i32x4*>(src); return; }
-        if (left >= 8 && wide == 1) {
-            *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
-            *reinterpret_cast<uint2*>(w + 2) = *reinterpret_cast<const uint2*>(src + 4);
-            return;
-        }
+    __device__ __forceinline__ void load(const T* src, int left) {
+        typedef uint32_t four __attribute__((ext_vector_type(4), aligned(2)));
+        if (left >= 8) { *reinterpret_cast<i32x4*>(w) = __builtin_bit_cast(i32x4, *reinterpret_cast<const four*>(src)); return; }
         const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = (2 * i < left ? (uint32_t)s[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)s[2 * i + 1] << 16 : 0u);
@@ -79,14 +74,11 @@ template <> __device__ __forceinline__ uint32_t Eight<_Float16>::bits32(uint32_t
 template <>
 struct Eight<float> {
     float v[8];
-    __device__ __forceinline__ void clear() {
+    __device__ __forceinline__ void load(const float* src, int left) {
+        if (left >= 8) {
+            const Vec4<float>::type a = *reinterpret_cast<const Vec4<float>::type*>(src), b = *reinterpret_cast<const Vec4<float>::type*>(src + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    }
-    __device__ __forceinline__ void load(const float* src, int left, int wide) {
-        if (left >= 8 && wide == 2) {
-            *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(src);
-            *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(src + 4);
+            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[i + 4] = b[i]; }
             return;
         }
 #pragma unroll
@@ -142,6 +134,17 @@ __device__ __forceinline__ uint2 encode_column(const Eight<T> x[8], int c, float
         for (int i = 0; i < 4; ++i) y.w[i] = __builtin_amdgcn_perm(x[2 * i + 1].w[c >> 1], x[2 * i].w[c >> 1], pick);
         return y.encode(scale);
     }
+}
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// Sixteen codes' products at a time on the bfloat16 matrix instruction, with the blocks' scales multiplied in: exact, since a code has four
+// significant bits and a scale none.
+__device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 }  // namespace gf

@@ -5,6 +5,9 @@
 
 namespace gf {
 
+// One block of 128 on either side: gf_fp8_thin (262221 rows, 96 -> 128, 32 bits, both directions: 179 us by the general path).
+static bool thin(uint64_t n, uint64_t k) { return n <= 128 && k <= 128; }
+
 static uint64_t blocks_of(uint64_t n) { return (n + 127) / 128; }
 
 // Hands out pieces of a buffer at multiples of 256 bytes; with base NULL it only measures.
@@ -32,11 +35,13 @@ struct Forward { uint8_t *x_codes, *x_scales, *w_codes, *w_scales, *parts; };
 static Forward forward_pieces(Pieces& p, const gf_fp8_linear_t& d) {
     Forward f = {};
     if (!d.w && d.m <= 16) return f;      // gf_fp8_rows needs nothing
-    f.x_codes = p.take(d.m * blocks_of(d.k) * 128);
-    f.x_scales = p.take(blocks_of(d.k) * d.m);
+    if (!thin(d.n, d.k)) {
+        f.x_codes = p.take(d.m * blocks_of(d.k) * 128);
+        f.x_scales = p.take(blocks_of(d.k) * d.m);
+        f.parts = p.take(gf_fp8_matmul_workspace_bytes(d.m, d.n, blocks_of(d.k)));
+    }
     if (d.w) f.w_codes = p.take(d.n * blocks_of(d.k) * 128);
     if (d.w && !d.keep_w) f.w_scales = p.take(blocks_of(d.n) * blocks_of(d.k));
-    f.parts = p.take(gf_fp8_matmul_workspace_bytes(d.m, d.n, blocks_of(d.k)));
     return f;
 }
 
@@ -45,6 +50,10 @@ struct Backward { uint8_t *row_codes, *row_scales, *col_codes, *col_scales, *par
 static Backward backward_pieces(Pieces& p, uint64_t m, uint64_t n, uint64_t k, bool dx, bool dw) {
     Backward b = {};
     uint64_t parts = 0;
+    if (thin(n, k)) {
+        if (dw) b.parts = p.take(gf_fp8_thin_workspace_bytes(m, n, k));
+        return b;
+    }
     if (dx) {
         b.row_codes = p.take(m * blocks_of(n) * 128);
         b.row_scales = p.take(blocks_of(n) * m);
@@ -92,7 +101,7 @@ GF_EXPORT int gf_fp8_linear(const gf_fp8_linear_t* d, void* stream) {
         const gf_fp8_rows_t r = {d->x, d->m, d->n, d->k, d->ldx, d->codes, d->scales, d->y, d->dtype, 0};
         return gf_fp8_rows(&r, stream);
     }
-    if (!d->workspace || ((d->keep_w || d->keep_x) && !d->saved)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: null buffer");
+    if ((!d->workspace && (d->w || !thin(d->n, d->k))) || ((d->keep_w || d->keep_x) && !d->saved)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: null buffer");
     if ((uintptr_t)d->workspace % 256 || (uintptr_t)d->saved % 256) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: buffers must start at multiples of 256 bytes");
     Pieces ps{(uint8_t*)d->saved}, pf{(uint8_t*)d->workspace};
     const Saved s = saved_pieces(ps, d->m, d->n, d->k, d->keep_w, d->keep_x);
@@ -106,6 +115,10 @@ GF_EXPORT int gf_fp8_linear(const gf_fp8_linear_t* d, void* stream) {
         w_codes = f.w_codes;
         w_scales = tiles;
     }
+    if (thin(d->n, d->k)) {
+        const gf_fp8_thin_t t = {d->x, d->ldx, d->m, d->n, d->k, w_codes, w_scales, d->y, s.x_codes, s.x_scales, d->dtype, 0};
+        return gf_fp8_thin(&t, stream);
+    }
     const gf_fp8_quantize_t q = {d->x, d->m, d->k, d->ldx, d->dtype, 0, f.x_codes, f.x_scales, s.x_codes, s.x_scales, nullptr, d->m, d->k};
     if (const int rc = gf_fp8_quantize(&q, stream)) return rc;
     const gf_fp8_matmul_t p = {{f.x_codes, f.x_scales, d->m, 0, 0}, {w_codes, w_scales, 0, kb, 1}, d->m, d->n, kb, d->y, d->dtype, 0, f.parts};
@@ -116,13 +129,17 @@ GF_EXPORT int gf_fp8_linear_backward(const gf_fp8_linear_backward_t* d, void* st
     if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear_backward: null descriptor");
     if (const int rc = size_error("gf_fp8_linear_backward", d->m, d->n, d->k)) return rc;
     if (!d->dx && !d->dw) return GF_OK;
-    if (!d->dy || !d->saved || !d->workspace) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear_backward: null pointer");
+    if (!d->dy || !d->saved || (!d->workspace && (d->dw || !thin(d->n, d->k)))) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear_backward: null pointer");
     if ((d->dx && !d->keep_w) || (d->dw && !d->keep_x)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear_backward: a gradient whose operand was not kept");
     if ((uintptr_t)d->workspace % 256 || (uintptr_t)d->saved % 256)
         return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear_backward: buffers must start at multiples of 256 bytes");
     Pieces ps{(uint8_t*)d->saved}, pb{(uint8_t*)d->workspace};
     const Saved s = saved_pieces(ps, d->m, d->n, d->k, d->keep_w, d->keep_x);
     const Backward b = backward_pieces(pb, d->m, d->n, d->k, d->dx != nullptr, d->dw != nullptr);
+    if (thin(d->n, d->k)) {
+        const gf_fp8_thin_backward_t t = {d->dy, d->lddy, d->m, d->n, d->k, s.w_codes, s.w_scales, s.x_codes, s.x_scales, d->dx, d->dw, b.parts, d->dtype, d->w_dtype};
+        return gf_fp8_thin_backward(&t, stream);
+    }
     const gf_fp8_quantize_t q = {d->dy, d->m, d->n, d->lddy, d->dtype, 0, b.row_codes, b.row_scales, b.col_codes, b.col_scales, nullptr, d->m, d->n};
     if (const int rc = gf_fp8_quantize(&q, stream)) return rc;
     if (d->dx) {      // b is w by columns: its scales are those of the tiles, transposed

@@ -5,6 +5,7 @@
 // they reach a lane does not matter as long as both operands have the same.
 #include "../common.hpp"
 #include "fp8.hpp"
+#include "fp8_join.hpp"
 #include "geneface_train_hip.h"
 
 namespace gf {
@@ -25,18 +26,8 @@ struct MatmulArgs {
 };
 
 typedef __attribute__((address_space(3))) void lds_t;
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 #define GF_FENCE __builtin_amdgcn_sched_barrier(0)      // the scheduler moves nothing across
-
-// Sixteen codes' products at a time on the bfloat16 matrix instruction, with the blocks' scales multiplied in: exact, since a code has four
-// significant bits and a scale none.
-__device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
-    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 // A workgroup of 2 x 2 waves makes a tile of 64 TM x 64 TN of the product, a wave TM x TN tiles of 32 x 32.
 //
@@ -218,7 +209,6 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
     static_assert(32 * PITCH <= BN * 128 && 32 * PITCH <= BM * 128, "staging");
     uint8_t* mine = wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1;
     T* out = (T*)d.out + (uint64_t)blockIdx.y * d.m * d.n;
-    const bool wide = ((uint64_t)d.n * sizeof(T)) % 16 == 0;      // (the output starts at a multiple of 16 bytes)
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -237,8 +227,9 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
             const i32x4 v = *reinterpret_cast<const i32x4*>(mine + r * PITCH + c * 16);
             if (row >= d.m || col >= d.n) continue;
             T* to = out + row * d.n + col;
-            if (wide) {
-                *reinterpret_cast<i32x4*>(to) = v;
+            if (col + EACH <= d.n) {
+                typedef int piece __attribute__((ext_vector_type(4), aligned(2)));
+                *reinterpret_cast<piece*>(to) = v;
             } else {
                 const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
@@ -252,37 +243,6 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
 template <typename T, bool EXACT, int TM, int TN>
 __global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN>(d); }
 
-// out = the sum of the splits' parts in a fixed order: a wave adds up every WAVES-th of them for 256 values, then the waves' sums are added.  Eight
-// loads are under way at a time: the parts of a tall product's weight gradient are hundreds, of few values each, and latency is all they cost.
-template <typename T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_join(const float* part, uint32_t splits, uint64_t count, T* out) {
-    __shared__ f32x4 sums[WAVES][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t i = ((uint64_t)blockIdx.x * 64 + lane) * 4;
-    const int left = i < count ? (int)min((uint64_t)4, count - i) : 0;
-    const bool wide = count % 4 == 0;
-    const float* at = part + (left ? i : 0);
-    f32x4 s = {0, 0, 0, 0};
-    for (uint32_t k = wave; k < splits; k += 8 * WAVES) {
-        float v[8][4];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) load4_of(at + min(k + u * WAVES, splits - 1) * count, k + u * WAVES < splits ? left : 0, wide, v[u]);
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] += v[u][e];
-    }
-    sums[wave][lane] = s;
-    __syncthreads();
-    if (wave) return;
-    float r[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] += sums[w][lane][e];
-    store4_of(out + (left ? i : 0), left, true, r);
-}
-
 // ---- a few rows ----------------------------------------------------------------------------------------------------------------------------
 // The weight's bytes bound it, and at the sizes it is called with, how many of them are under way at once.  A wave takes 16 rows of the weight (one row of
 // codes is 128 bytes a block: whole cache lines, straight into registers) and every 16th block, two blocks at a time, all loads before the first
@@ -292,7 +252,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_join(const float* part, uint32_t
 constexpr int kRowWaves = 16, kRowBlocks = 2;
 
 template <typename T>
-__global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d, const int wide) {
+__global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d) {
     __shared__ f32x4 part[kRowWaves][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const uint64_t n0 = (uint64_t)blockIdx.x * 16;
@@ -320,7 +280,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d, 
             for (int i = 0; i < 4; ++i) {
                 const uint64_t k = (uint64_t)(b0 + u * kRowWaves) * 128 + q * 32 + 8 * i;
                 const int left = there && k < d.k ? (int)min((uint64_t)8, d.k - k) : 0;
-                v[u][i].load(x + (left ? k : 0), left, wide);
+                v[u][i].load(x + (left ? k : 0), left);
             }
 #pragma unroll
         for (int u = 0; u < kRowBlocks; ++u) {
@@ -395,9 +355,7 @@ static void launch_matmul(MatmulArgs a, const Plan& p, void* workspace, hipStrea
     a.out = workspace;
     launch_tiles<float, exact>(a, p, s);
     const uint64_t count = (uint64_t)a.m * a.n;
-    const uint32_t grid = (uint32_t)((count + 255) / 256);
-    if (p.splits > 16) k_join<T, 16><<<grid, 1024, 0, s>>>((const float*)workspace, p.splits, count, out);
-    else k_join<T, 4><<<grid, 256, 0, s>>>((const float*)workspace, p.splits, count, out);
+    launch_join<T>((const float*)workspace, p.splits, count, out, s);
 }
 
 static const char* operand_error(const gf_fp8_operand_t& o, uint64_t rows) {
@@ -426,7 +384,6 @@ GF_EXPORT int gf_fp8_matmul(const gf_fp8_matmul_t* d, void* stream) {
     if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null descriptor");
     if (d->m == 0 || d->n == 0) return GF_OK;
     if (!d->out) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null output");
-    if ((uintptr_t)d->out % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: the output must start at a multiple of 16 bytes");
     if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: unknown dtype %u", d->dtype);
     if (d->blocks == 0) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: no blocks to add up");
     if (const char* e = operand_error(d->a, d->m)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: a: %s", e);
@@ -457,13 +414,10 @@ GF_EXPORT int gf_fp8_rows(const gf_fp8_rows_t* d, void* stream) {
     if (d->k >> 31) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: matrix too large");
     if ((uintptr_t)d->codes % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: codes must start at a multiple of 16 bytes");
     if ((d->n + 15) / 16 >> 31) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: matrix too large");
-    const uint64_t size = d->dtype == F32 ? 4 : 2;
-    const uint64_t at = (uintptr_t)d->x | (d->m > 1 ? d->ldx * size : 0);
-    const int wide = at % 16 == 0 ? 2 : size == 2 && at % 8 == 0 ? 1 : 0;
     const uint32_t grid = (uint32_t)((d->n + 15) / 16);
     const hipStream_t s = gf_stream(stream);
-    if (d->dtype == F32) k_rows<float><<<grid, 64 * kRowWaves, 0, s>>>(*d, wide);
-    else if (d->dtype == BF16) k_rows<__bf16><<<grid, 64 * kRowWaves, 0, s>>>(*d, wide);
-    else k_rows<_Float16><<<grid, 64 * kRowWaves, 0, s>>>(*d, wide);
+    if (d->dtype == F32) k_rows<float><<<grid, 64 * kRowWaves, 0, s>>>(*d);
+    else if (d->dtype == BF16) k_rows<__bf16><<<grid, 64 * kRowWaves, 0, s>>>(*d);
+    else k_rows<_Float16><<<grid, 64 * kRowWaves, 0, s>>>(*d);
     return gf_check_launch("gf_fp8_rows");
 }

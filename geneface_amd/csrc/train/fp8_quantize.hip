@@ -13,7 +13,7 @@ namespace gf {
 constexpr int kTile = 128;
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, const uint32_t blocks_r, const uint32_t blocks_c, const int wide) {
+__global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, const uint32_t blocks_r, const uint32_t blocks_c) {
     __shared__ uint32_t most[4][kTile];                                // a wave's largest magnitudes by column
     __shared__ __align__(16) uint8_t turned[kTile * kTile];
     const int t = threadIdx.x, j = t & 15, g = t >> 4, wave = t >> 6;  // columns 8j..8j+7 of the tile, rows 8g..8g+7
@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, con
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const bool there = r0 + r < d.rows && left > 0;
-        x[r].load(src + (there ? (r0 + r) * d.ld + c0 : 0), there ? left : 0, wide);
+        x[r].load(src + (there ? (r0 + r) * d.ld + c0 : 0), there ? left : 0);
     }
     uint32_t rm[8], cm[8];
 #pragma unroll
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, con
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d, const uint32_t blocks_c, const int wide) {
+__global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d, const uint32_t blocks_c) {
     const int j = threadIdx.x & 15, g = threadIdx.x >> 4;
     const uint32_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
     const uint64_t r0 = (uint64_t)br * 32 + 2 * g, c0 = (uint64_t)bc * kTile + 8 * j;
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const bool there = r0 + r < d.rows && left > 0;
-        x[r].load((const T*)d.src + (there ? (r0 + r) * d.ld + c0 : 0), there ? left : 0, wide);
+        x[r].load((const T*)d.src + (there ? (r0 + r) * d.ld + c0 : 0), there ? left : 0);
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -115,9 +115,9 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d
 }
 
 template <typename T>
-static void launch_quantize(const gf_fp8_quantize_t& d, uint64_t rb, uint64_t cb, int wide, hipStream_t s) {
-    if (!d.col_codes && !d.tiles) k_quantize_rows<T><<<(uint32_t)((d.rows + 31) / 32 * cb), 256, 0, s>>>(d, (uint32_t)cb, wide);
-    else k_quantize<T><<<(uint32_t)(rb * cb), 256, 0, s>>>(d, (uint32_t)rb, (uint32_t)cb, wide);
+static void launch_quantize(const gf_fp8_quantize_t& d, uint64_t rb, uint64_t cb, hipStream_t s) {
+    if (!d.col_codes && !d.tiles) k_quantize_rows<T><<<(uint32_t)((d.rows + 31) / 32 * cb), 256, 0, s>>>(d, (uint32_t)cb);
+    else k_quantize<T><<<(uint32_t)(rb * cb), 256, 0, s>>>(d, (uint32_t)rb, (uint32_t)cb);
 }
 
 }  // namespace gf
@@ -136,11 +136,9 @@ GF_EXPORT int gf_fp8_quantize(const gf_fp8_quantize_t* d, void* stream) {
         return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: scale pitch too small");
     const uint64_t rb = (d->rows + kTile - 1) / kTile, cb = (d->cols + kTile - 1) / kTile;
     if (rb > 0x1fffffffull || cb > 0x1fffffffull / rb) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: matrix too large");
-    const uint64_t size = d->dtype == F32 ? 4 : 2, at = (uintptr_t)d->src | d->ld * size;
-    const int wide = at % 16 == 0 ? 2 : size == 2 && at % 8 == 0 ? 1 : 0;
     const hipStream_t s = gf_stream(stream);
-    if (d->dtype == F32) launch_quantize<float>(*d, rb, cb, wide, s);
-    else if (d->dtype == BF16) launch_quantize<__bf16>(*d, rb, cb, wide, s);
-    else launch_quantize<_Float16>(*d, rb, cb, wide, s);
+    if (d->dtype == F32) launch_quantize<float>(*d, rb, cb, s);
+    else if (d->dtype == BF16) launch_quantize<__bf16>(*d, rb, cb, s);
+    else launch_quantize<_Float16>(*d, rb, cb, s);
     return gf_check_launch("gf_fp8_quantize");
 }

@@ -109,7 +109,7 @@ typedef struct {
     uint64_t stride_row, stride_block;
 } gf_fp8_operand_t;
 
-/* out [m, n] of `dtype` (contiguous, at a multiple of 16 bytes) = a [m, 128 blocks] b [n, 128 blocks]^T, added up in 32 bits; blocks <= 65535.
+/* out [m, n] of `dtype` (contiguous) = a [m, 128 blocks] b [n, 128 blocks]^T, added up in 32 bits; blocks <= 65535.
  * workspace: gf_fp8_matmul_workspace_bytes(m, n, blocks) device bytes of this call's own (NULL where that is 0). */
 typedef struct {
     gf_fp8_operand_t a, b;
@@ -134,6 +134,38 @@ typedef struct {
     uint32_t _pad;
 } gf_fp8_rows_t;
 int gf_fp8_rows(const gf_fp8_rows_t* desc, void* stream);
+
+/* The same products where n and k are at most 128, a block each, in one launch over the rows: y [m, n] = Q_row(x) w^T with w as codes [n, 128] and the
+ * byte of its one scale; x by columns is left in col_codes [k, up(m)] and col_scales [up(m)/128, k], or both are NULL. */
+typedef struct {
+    const void* x;
+    uint64_t ldx, m, n, k;
+    const uint8_t* codes;
+    const uint8_t* scale;
+    void* y;
+    uint8_t* col_codes;
+    uint8_t* col_scales;
+    uint32_t dtype;
+    uint32_t _pad;
+} gf_fp8_thin_t;
+int gf_fp8_thin(const gf_fp8_thin_t* desc, void* stream);
+
+/* dx [m, k] of dtype (or NULL) from the weight by columns, codes [k, 128] and the byte of its scale; dw [n, k] of w_dtype (or NULL) from x by columns
+ * as gf_fp8_thin left it.  workspace: gf_fp8_thin_workspace_bytes(m, n, k) device bytes of this call's own, where dw is given. */
+typedef struct {
+    const void* dy;
+    uint64_t lddy, m, n, k;
+    const uint8_t* codes;
+    const uint8_t* scale;
+    const uint8_t* col_codes;
+    const uint8_t* col_scales;
+    void* dx;
+    void* dw;
+    void* workspace;
+    uint32_t dtype, w_dtype;
+} gf_fp8_thin_backward_t;
+uint64_t gf_fp8_thin_workspace_bytes(uint64_t m, uint64_t n, uint64_t k);
+int gf_fp8_thin_backward(const gf_fp8_thin_backward_t* desc, void* stream);
 
 /* A linear layer, y [m, n] = Q_row(x) Q_tile(w)^T, and its gradients dx [m, k] = Q_row(dy) Q_tile(w), dw [n, k] = Q_col(dy)^T Q_col(x), each as one
  * call that enqueues all its launches.  x, dy: ldx / lddy values from row to row.  The weight is given as values w [n, k] of w_dtype (ldw values from

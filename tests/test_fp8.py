@@ -91,7 +91,6 @@ def test_the_library_refuses_bad_descriptors(hip_lib):
     refused(hip_lib.gf_fp8_matmul(None, None), b"null")
     assert hip_lib.gf_fp8_matmul(m(m=0), None) == 0 and hip_lib.gf_fp8_matmul(m(n=0), None) == 0
     refused(hip_lib.gf_fp8_matmul(m(out=0), None), b"null output")
-    refused(hip_lib.gf_fp8_matmul(m(out=8), None), b"multiple of 16")
     refused(hip_lib.gf_fp8_matmul(m(dtype=3), None), b"dtype")
     refused(hip_lib.gf_fp8_matmul(m(blocks=0), None), b"no blocks")
     refused(hip_lib.gf_fp8_matmul(m(a_codes=0), None), b"a: null")
@@ -101,11 +100,11 @@ def test_the_library_refuses_bad_descriptors(hip_lib):
     refused(hip_lib.gf_fp8_matmul(m(blocks=1 << 16), None), b"too large")
     refused(hip_lib.gf_fp8_matmul(m(blocks=1000), None), b"workspace")
     assert hip_lib.gf_fp8_matmul_workspace_bytes(300, 300, 1000) % (4 * 300 * 300) == 0 and hip_lib.gf_fp8_matmul_workspace_bytes(300, 300, 1) == 0
-    f = lambda **k: fp8.GfFp8Linear(**{"x": 16, "ldx": 5, "w": 16, "ldw": 5, "m": 300, "n": 7, "k": 5, "y": 16, "workspace": 256, "saved": 256, "keep_x": 1, **k})      # noqa: E731
+    f = lambda **k: fp8.GfFp8Linear(**{"x": 16, "ldx": 150, "w": 16, "ldw": 150, "m": 300, "n": 200, "k": 150, "y": 16, "workspace": 256, "saved": 256, "keep_x": 1, **k})      # noqa: E731
     refused(hip_lib.gf_fp8_linear_plan(None), b"null")
     refused(hip_lib.gf_fp8_linear_plan(C.byref(f(k=0))), b"empty")
     p = f(keep_w=1)
-    assert hip_lib.gf_fp8_linear_plan(C.byref(p)) == 0 and p.saved_bytes >= 5 * 128 + 1 + 5 * 384 + 15 and p.workspace_bytes >= 300 * 128 and p.backward_bytes >= 300 * 128 + 7 * 384
+    assert hip_lib.gf_fp8_linear_plan(C.byref(p)) == 0 and p.saved_bytes >= 150 * 256 + 4 + 150 * 384 + 3 * 150 and p.workspace_bytes >= 300 * 256 and p.backward_bytes >= 300 * 256 + 200 * 384
     refused(hip_lib.gf_fp8_linear(None, None), b"null")
     for change in (dict(x=None), dict(y=None), dict(w=None)):
         refused(hip_lib.gf_fp8_linear(C.byref(f(**change)), None), b"null pointer")
@@ -114,13 +113,27 @@ def test_the_library_refuses_bad_descriptors(hip_lib):
     refused(hip_lib.gf_fp8_linear(C.byref(f(saved=None)), None), b"null buffer")
     refused(hip_lib.gf_fp8_linear(C.byref(f(workspace=16)), None), b"multiples of 256")
     refused(hip_lib.gf_fp8_linear(C.byref(f(w=None, codes=16, scales=16)), None), b"no backward")
-    g = lambda **k: C.byref(fp8.GfFp8LinearBackward(**{"dy": 16, "lddy": 7, "saved": 256, "m": 300, "n": 7, "k": 5, "dx": 16, "dw": 16, "workspace": 256, "keep_w": 1, "keep_x": 1, **k}))      # noqa: E731
+    g = lambda **k: C.byref(fp8.GfFp8LinearBackward(**{"dy": 16, "lddy": 200, "saved": 256, "m": 300, "n": 200, "k": 150, "dx": 16, "dw": 16, "workspace": 256, "keep_w": 1, "keep_x": 1, **k}))      # noqa: E731
     refused(hip_lib.gf_fp8_linear_backward(None, None), b"null")
     assert hip_lib.gf_fp8_linear_backward(g(dx=None, dw=None), None) == 0
     refused(hip_lib.gf_fp8_linear_backward(g(dy=None), None), b"null")
     refused(hip_lib.gf_fp8_linear_backward(g(keep_x=0), None), b"not kept")
     refused(hip_lib.gf_fp8_linear_backward(g(keep_w=0), None), b"not kept")
     refused(hip_lib.gf_fp8_linear_backward(g(saved=16), None), b"multiples of 256")
+    thin = ["x", "ldx", "m", "n", "k", "codes", "scale", "y", "col_codes", "col_scales", "dtype"]
+    t = lambda **k: (C.c_uint64 * 11)(*[{**dict(x=16, ldx=5, m=300, n=7, k=5, codes=16, scale=16, y=16, col_codes=16, col_scales=16), **k}.get(n, 0) for n in thin])      # noqa: E731
+    refused(hip_lib.gf_fp8_thin(None, None), b"null")
+    for change, word in ((dict(n=129), b"1 to 128"), (dict(k=0), b"1 to 128"), (dict(m=0), b"rows"), (dict(dtype=3), b"dtype"), (dict(x=0), b"null"), (dict(scale=0), b"null"),
+                         (dict(col_scales=0), b"null"), (dict(codes=24), b"multiple of 16"), (dict(ldx=4), b"ldx < k")):
+        refused(hip_lib.gf_fp8_thin(t(**change), None), word)
+    back = ["dy", "lddy", "m", "n", "k", "codes", "scale", "col_codes", "col_scales", "dx", "dw", "workspace", "dtype"]
+    b = lambda **k: (C.c_uint64 * 13)(*[{**{n: 16 for n in back if n != "dtype"}, "lddy": 7, "m": 300, "n": 7, "k": 5, **k}.get(n, 0) for n in back])      # noqa: E731
+    refused(hip_lib.gf_fp8_thin_backward(None, None), b"null")
+    assert hip_lib.gf_fp8_thin_backward(b(dx=0, dw=0), None) == 0
+    for change, word in ((dict(n=129), b"1 to 128"), (dict(m=1 << 31), b"rows"), (dict(dy=0), b"null"), (dict(codes=0), b"null"), (dict(col_codes=0), b"null"),
+                         (dict(workspace=0), b"null"), (dict(lddy=6), b"lddy < n"), (dict(dtype=7 << 32), b"dtype"), (dict(dtype=7), b"dtype")):
+        refused(hip_lib.gf_fp8_thin_backward(b(**change), None), word)
+    assert hip_lib.gf_fp8_thin_workspace_bytes(300, 7, 5) == 3 * 7 * 5 * 4 and hip_lib.gf_fp8_thin_workspace_bytes(300, 129, 5) == 0
     rows = ["x", "m", "n", "k", "ldx", "codes", "scales", "out", "dtype"]
     r = lambda **k: (C.c_uint64 * 9)(*[{**{"x": 16, "m": 3, "n": 7, "k": 5, "ldx": 5, "codes": 16, "scales": 16, "out": 16}, **k}.get(n, 0) for n in rows])      # noqa: E731
     refused(hip_lib.gf_fp8_rows(None, None), b"null")
