@@ -7,6 +7,8 @@
 #include "fp8.hpp"
 #include "fp8_join.hpp"
 #include "geneface_train_hip.h"
+#include <type_traits>
+#include <utility>
 
 namespace gf {
 
@@ -29,22 +31,39 @@ typedef __attribute__((address_space(3))) void lds_t;
 
 #define GF_FENCE __builtin_amdgcn_sched_barrier(0)      // the scheduler moves nothing across
 
+// An array in LDS of its own for each TAG: the compiler then knows that a load into one is not what a read of another waits for.
+template <int BYTES, int TAG>
+__device__ __forceinline__ uint8_t* lds_array() {
+    __shared__ __align__(16) uint8_t bytes[BYTES];
+    return bytes;
+}
+
+template <int N> using Const = std::integral_constant<int, N>;
+template <int N, typename F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) { (f(Const<I>{}), ...); }
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) { each<N>(f, std::make_integer_sequence<int, N>{}); }      // f(Const<0>), f(Const<1>), ..
+
+// s_waitcnt: at most vm loads and lgkm LDS reads still under way
+constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 | (vm >> 4) << 14; }
+
 // A workgroup of 2 x 2 waves makes a tile of 64 TM x 64 TN of the product, a wave TM x TN tiles of 32 x 32.
 //
-// Blocks of codes come straight from memory to LDS, two of them at a time (the buffer descriptor ends with the tile's last row: rows behind it read as
-// zero).  Row r is 128 bytes, its 16-byte piece c at place c ^ ((r >> 1) & 7), so that the same piece of any 16 consecutive rows lies on
+// Blocks of codes come straight from memory to LDS, STAGES of them under way (the buffer descriptor ends with the tile's last row: rows behind it
+// read as zero).  Row r is 128 bytes, its 16-byte piece c at place c ^ ((r >> 1) & 7), so that the same piece of any 16 consecutive rows lies on
 // different banks.  A step multiplies one block in two halves of 64, and the fragments of a half are read from LDS while the half before it is
-// multiplied, so the matrix unit waits for nothing but the one barrier of a step: behind it everyone has read the block, whose place the block after
-// the next is then loaded into.  With one wave on each SIMD there is nobody else to fill a gap, hence the interleaving by hand (weave): one
+// multiplied, so the matrix unit waits for nothing but the one barrier of a step: behind it everyone has read the block, whose place the block
+// STAGES further on is then loaded into.  With one wave on each SIMD there is nobody else to fill a gap, hence the interleaving by hand (weave): one
 // LDS read and one load beside each matrix instruction.
 //
 // EXACT: the 8-bit matrix instructions add the products of one instruction with about 17 bits (measured: 1.6e-5 of the result for normal values,
 // 5.6e-5 for log-normal ones, against 1e-7 of the bfloat16 instruction).  That is below half a step of a 16-bit result (2^-9, 2^-12), and not what a
 // 32-bit one should carry: for those the codes are widened to bfloat16 on the way out of LDS.
-template <typename T, bool EXACT, int TM, int TN>
+template <typename T, bool EXACT, int TM, int TN, int STAGES>
 __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
     constexpr int BM = 64 * TM, BN = 64 * TN, LA = BM / 32, LB = BN / 32;      // 32 rows of 128 bytes a load of the workgroup
-    __shared__ __align__(16) uint8_t a0[BM * 128], a1[BM * 128], b0[BN * 128], b1[BN * 128];      // four arrays: the compiler tells them apart
+    auto stage_a = [](auto j) __attribute__((always_inline)) { return lds_array<BM * 128, decltype(j)::value>(); };
+    auto stage_b = [](auto j) __attribute__((always_inline)) { return lds_array<BN * 128, 16 + decltype(j)::value>(); };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave >> 1, wc = wave & 1;
 
     // Workgroups go to the 8 XCDs in turn.  Each XCD gets a contiguous range of tiles, walked in bands of 8 rows of tiles, so that what its
@@ -54,8 +73,8 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
         const uint32_t total = d.tiles_m * d.tiles_n, xcd = blockIdx.x & 7, full = total / 8, rest = total % 8;
         const uint32_t t = xcd * full + min(xcd, rest) + (blockIdx.x >> 3), band = t / (8 * d.tiles_n), in = t % (8 * d.tiles_n);
         const uint32_t high = min(8u, d.tiles_m - band * 8);
-        tile_m = band * 8 + in % high;
-        tile_n = in / high;
+        tile_m = __builtin_amdgcn_readfirstlane(band * 8 + in % high);
+        tile_n = __builtin_amdgcn_readfirstlane(in / high);
     }
     const uint64_t m0 = (uint64_t)tile_m * BM, n0 = (uint64_t)tile_n * BN;
     const uint32_t kb0 = blockIdx.y * d.per_split, nb = min(d.blocks, kb0 + d.per_split) - kb0, width = d.blocks * 128;
@@ -77,7 +96,7 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
         for (int i = 0; i < LB; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_t*)(B + (i * 4 + wave) * 1024), 16, off + i * 32 * width, at, 0, 0);
     };
 
-    // Scales: a byte for each row of a fragment, read two steps before it is used.
+    // Scales: a byte for each row of a fragment, read at least STAGES - 1 steps before it is used.
     const uint64_t step_a = d.a.step(), step_b = d.b.step();
     const uint8_t *sa = d.a.scales + d.a.at(m0) + kb0 * step_a, *sb = d.b.scales + d.b.at(n0) + kb0 * step_b;
     uint32_t ca[TM], cb[TN];
@@ -85,13 +104,27 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
     for (int i = 0; i < TM; ++i) ca[i] = (uint32_t)d.a.at(min((uint32_t)((wr * TM + i) * 32 + (lane & 31)), (uint32_t)(d.m - 1 - m0)));
 #pragma unroll
     for (int i = 0; i < TN; ++i) cb[i] = (uint32_t)d.b.at(min((uint32_t)((wc * TN + i) * 32 + (lane & 31)), (uint32_t)(d.n - 1 - n0)));
-    auto scales = [&](int* p, int* q, uint32_t kb) __attribute__((always_inline)) {
-        const uint32_t at = min(kb, nb - 1);
-        const uint8_t *u = sa + at * step_a, *v = sb + at * step_b;
+    int xa[STAGES][TM], xb[STAGES][TN], nxa[STAGES][TM], nxb[STAGES][TN];      // of the STAGES blocks at hand, and of the next
+    auto read_scales = [&](uint32_t kb) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) p[i] = u[ca[i]];
+        for (int j = 0; j < STAGES; ++j) {
+            const uint32_t at = min(kb + j, nb - 1);
+            const uint8_t *u = sa + at * step_a, *v = sb + at * step_b;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) q[i] = v[cb[i]];
+            for (int i = 0; i < TM; ++i) nxa[j][i] = u[ca[i]];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) nxb[j][i] = v[cb[i]];
+        }
+    };
+    auto take_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < STAGES; ++j) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) xa[j][i] = nxa[j][i];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) xb[j][i] = nxb[j][i];
+        }
+        GF_FENCE;
     };
 
     // Fragments: lane l holds row l % 32 and 32 of the half's 64 codes, the pieces 4 half + 2 (l / 32) and the next.
@@ -143,71 +176,69 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
                     acc[i][k] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[k], fa[i], acc[i][k], 0, 0, 0, q[k], 0, p[i]);
         }
     };
-    auto weave = [&](bool loads) __attribute__((always_inline)) {
+    auto weave = [&](auto loads) __attribute__((always_inline)) {
         constexpr int MF = TM * TN * (EXACT ? 4 : 1), DS = 2 * (TM + TN), LD = LA + LB;
         constexpr int per_ds = DS > MF ? DS / MF : 1, per_ld = LD > MF ? LD / MF : 1;
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                    // a matrix instruction,
-            if (loads) __builtin_amdgcn_sched_group_barrier(0x010, per_ld, 0);    // a load,
-            __builtin_amdgcn_sched_group_barrier(0x100, per_ds, 0);               // a read from LDS
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                          // a matrix instruction,
+            if constexpr (decltype(loads)::value) __builtin_amdgcn_sched_group_barrier(0x010, per_ld, 0);    // a load,
+            __builtin_amdgcn_sched_group_barrier(0x100, per_ds, 0);                                     // a read from LDS
         }
     };
 
     i32x8 fa0[TM], fb0[TN], fa1[TM], fb1[TN];
-    int xa[TM], xb[TN], ya[TM], yb[TN], nxa[TM], nxb[TN], nya[TM], nyb[TN];
-    auto step = [&](uint8_t* A, uint8_t* B, const uint8_t* A2, const uint8_t* B2, const int* p, const int* q, uint32_t kb) __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0): the first half's fragments
+    auto step = [&](auto j, uint32_t kb) __attribute__((always_inline)) {
+        constexpr int J = decltype(j)::value;
+        uint8_t *A = stage_a(j), *B = stage_b(j);
+        const uint8_t *A2 = stage_a(Const<(J + 1) % STAGES>{}), *B2 = stage_b(Const<(J + 1) % STAGES>{});
+        __builtin_amdgcn_s_waitcnt(waitcnt(63, 0));      // the first half's fragments
         GF_FENCE;
         read(A, B, 1, fa1, fb1);
-        multiply(fa0, fb0, p, q);
-        weave(false);
+        multiply(fa0, fb0, xa[J], xb[J]);
+        weave(Const<0>{});
         GF_FENCE;
-        __builtin_amdgcn_s_waitcnt(0x0070);      // vmcnt(0), lgkmcnt(0): the next block is there, and this one is read
+        // The next block is there and this one is read.  STAGES - 2 blocks were asked for behind the next one; scales that were asked for in between
+        // only make the wait a longer one.
+        __builtin_amdgcn_s_waitcnt(waitcnt((STAGES - 2) * (LA + LB), 0));
         __builtin_amdgcn_s_barrier();
         GF_FENCE;
-        load(A, B, kb + 2);
+        if constexpr (J == 0) {
+            read_scales(kb + STAGES);
+            GF_FENCE;
+        }
+        load(A, B, kb + STAGES);
         read(A2, B2, 0, fa0, fb0);
-        multiply(fa1, fb1, p, q);
-        weave(true);
+        multiply(fa1, fb1, xa[J], xb[J]);
+        weave(Const<1>{});
         GF_FENCE;
     };
-    auto rotate = [&](uint32_t kb) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) { xa[i] = nxa[i]; ya[i] = nya[i]; }
-#pragma unroll
-        for (int i = 0; i < TN; ++i) { xb[i] = nxb[i]; yb[i] = nyb[i]; }
-        scales(nxa, nxb, kb + 2);
-        scales(nya, nyb, kb + 3);
-        GF_FENCE;
-    };
-    load(a0, b0, 0);
-    scales(nxa, nxb, 0);
-    scales(nya, nyb, 1);
-    load(a1, b1, 1);
-    __builtin_amdgcn_s_waitcnt(0x0f70);
+
+    read_scales(0);
+    GF_FENCE;
+    each<STAGES>([&](auto j) __attribute__((always_inline)) { load(stage_a(j), stage_b(j), decltype(j)::value); });
+    __builtin_amdgcn_s_waitcnt(waitcnt((STAGES - 1) * (LA + LB), 0));
     __builtin_amdgcn_s_barrier();
     GF_FENCE;
-    read(a0, b0, 0, fa0, fb0);
+    read(stage_a(Const<0>{}), stage_b(Const<0>{}), 0, fa0, fb0);
     uint32_t kb = 0;
-    for (; kb + 1 < nb; kb += 2) {
-        rotate(kb);
-        step(a0, b0, a1, b1, xa, xb, kb);
-        step(a1, b1, a0, b0, ya, yb, kb + 1);
+    for (; kb + STAGES <= nb; kb += STAGES) {
+        take_scales();
+        each<STAGES>([&](auto j) __attribute__((always_inline)) { step(j, kb + decltype(j)::value); });
     }
-    if (nb & 1) {
-        rotate(kb);
-        read(a0, b0, 1, fa1, fb1);
-        multiply(fa0, fb0, xa, xb);
-        multiply(fa1, fb1, xa, xb);
+    if (kb < nb) {
+        take_scales();
+        each<STAGES - 1>([&](auto j) __attribute__((always_inline)) {
+            if (kb + decltype(j)::value < nb) step(j, kb + decltype(j)::value);
+        });
     }
-    __builtin_amdgcn_s_waitcnt(0x0070);      // no load is under way and nobody reads any more: LDS is free
+    __builtin_amdgcn_s_waitcnt(waitcnt(0, 0));      // no load is under way and nobody reads any more: LDS is free
     __builtin_amdgcn_s_barrier();
 
     // 32 rows of the wave's part at a time through LDS, so that a row leaves in pieces of 16 bytes.
     constexpr int COLS = 32 * TN, PITCH = COLS * (int)sizeof(T) + 16, EACH = 16 / (int)sizeof(T), PIECES = COLS / EACH;
     static_assert(32 * PITCH <= BN * 128 && 32 * PITCH <= BM * 128, "staging");
-    uint8_t* mine = wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? b0 : b1;
+    uint8_t* mine = wave == 0 ? stage_a(Const<0>{}) : wave == 1 ? stage_a(Const<1>{}) : wave == 2 ? stage_b(Const<0>{}) : stage_b(Const<1>{});
     T* out = (T*)d.out + (uint64_t)blockIdx.y * d.m * d.n;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
@@ -218,7 +249,7 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
                 const float v[4] = {acc[i][k][4 * g], acc[i][k][4 * g + 1], acc[i][k][4 * g + 2], acc[i][k][4 * g + 3]};
                 store4((T*)(mine + (lane & 31) * PITCH) + k * 32 + g * 8 + (lane >> 5) * 4, v);
             }
-        __builtin_amdgcn_s_waitcnt(0xc07f);      // the wave's own stores (it alone reads them)
+        __builtin_amdgcn_s_waitcnt(waitcnt(63, 0));      // the wave's own stores (it alone reads them)
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int q = 0; q < 32 * PIECES / 64; ++q) {
@@ -240,8 +271,8 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
     }
 }
 
-template <typename T, bool EXACT, int TM, int TN>
-__global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN>(d); }
+template <typename T, bool EXACT, int TM, int TN, int STAGES>
+__global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN, STAGES>(d); }
 
 // ---- a few rows ----------------------------------------------------------------------------------------------------------------------------
 // The weight's bytes bound it, and at the sizes it is called with, how many of them are under way at once.  A wave takes 16 rows of the weight (one row of
@@ -332,7 +363,7 @@ static Plan plan_of(uint64_t m, uint64_t n, uint64_t blocks) {
     p.tiles_m = (uint32_t)((m + p.edge - 1) / p.edge);
     p.tiles_n = (uint32_t)((n + p.edge - 1) / p.edge);
     const uint64_t t = tiles(p.edge);
-    uint64_t s = t >= 256 || p.edge == 256 ? 1 : 512 / t;
+    uint64_t s = t >= 256 || p.edge == 256 ? 1 : 256 / t;
     if (s > blocks / 4) s = blocks / 4;
     if (s < 1) s = 1;
     p.per_split = (uint32_t)((blocks + s - 1) / s);
@@ -343,8 +374,8 @@ static Plan plan_of(uint64_t m, uint64_t n, uint64_t blocks) {
 template <typename T, bool EXACT>
 static void launch_tiles(const MatmulArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid(p.tiles_m * p.tiles_n, p.splits);
-    if (p.edge == 256) k_matmul<T, EXACT, 4, 4><<<grid, 256, 0, s>>>(a);
-    else k_matmul<T, EXACT, 2, 2><<<grid, 256, 0, s>>>(a);
+    if (p.edge == 256) k_matmul<T, EXACT, 4, 4, 2><<<grid, 256, 0, s>>>(a);
+    else k_matmul<T, EXACT, 2, 2, 4><<<grid, 256, 0, s>>>(a);
 }
 
 template <typename T>
