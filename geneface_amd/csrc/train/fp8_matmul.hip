@@ -275,67 +275,71 @@ template <typename T, bool EXACT, int TM, int TN, int STAGES>
 __global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN, STAGES>(d); }
 
 // ---- a few rows ----------------------------------------------------------------------------------------------------------------------------
-// The weight's bytes bound it, and at the sizes it is called with, how many of them are under way at once.  A wave takes 16 rows of the weight (one row of
-// codes is 128 bytes a block: whole cache lines, straight into registers) and every 16th block, two blocks at a time, all loads before the first
-// use; 16 waves of a workgroup share the rows and add up through LDS.  A wave brings its blocks of x to 8 bits itself, in the registers that the
-// matrix instruction takes them from: lane l holds row l % 16 of x, values (l / 16) * 32 .. + 31 of the block, so the block's largest magnitude
-// is two exchanges away.
-constexpr int kRowWaves = 16, kRowBlocks = 2;
+// The weight's bytes bound it, and at the sizes it is called with, how many of them are under way at once and how long the way to the first product is.
+// A wave takes 16 rows of the weight (one row of codes is 128 bytes a block: whole cache lines, straight into registers) and every 16th block, two
+// blocks ahead; 16 waves of a workgroup share the rows and add up through LDS.  While the first blocks of the weight are under way the workgroup
+// brings x to 8 bits in LDS, 16 lanes to a block of a row: 8 values a lane, as few as they can be shared out.
+constexpr int kRowWaves = 16, kRowBlocks = 2, kRowBytes = 128 * 1024;      // codes of x at a time
 
 template <typename T>
 __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d) {
     __shared__ f32x4 part[kRowWaves][64];
+    __shared__ __align__(16) uint8_t codes[kRowBytes + 16 * 16];
+    __shared__ uint8_t bytes[kRowBytes / 128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const uint64_t n0 = (uint64_t)blockIdx.x * 16;
-    const uint32_t blocks = (uint32_t)((d.k + 127) / 128);
+    const uint32_t blocks = (uint32_t)((d.k + 127) / 128), rows = (uint32_t)d.m;
     const uint64_t row = min(n0 + r, d.n - 1);
     const uint8_t* w = d.codes + row * blocks * 128 + q * 32;
     const uint8_t* ws = d.scales + (row >> 7) * blocks;
-    const T* x = (const T*)d.x + min((uint64_t)r, d.m - 1) * d.ldx;
-    const bool there = (uint32_t)r < d.m;
+    const uint32_t room = kRowBytes / 128 / rows;                          // blocks of x that fit
     f32x4 acc = {0, 0, 0, 0};
-    for (uint32_t b0 = wave; b0 < blocks; b0 += kRowWaves * kRowBlocks) {
+    for (uint32_t c0 = 0; c0 < blocks; c0 += room) {
+        const uint32_t here = min(room, blocks - c0), pitch = here * 128 + 16;      // 16: the rows' same piece on different banks
         i32x4 lo[kRowBlocks], hi[kRowBlocks];
         int sw[kRowBlocks];
-        Eight<T> v[kRowBlocks][4];
+        auto ahead = [&](uint32_t b0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kRowBlocks; ++u) {      // behind the last block: that one again, with an x of zeros
-            const uint64_t b = min(b0 + u * kRowWaves, blocks - 1);
-            lo[u] = *reinterpret_cast<const i32x4*>(w + b * 128);
-            hi[u] = *reinterpret_cast<const i32x4*>(w + b * 128 + 16);
-            sw[u] = ws[b];
+            for (int u = 0; u < kRowBlocks; ++u) {
+                const uint64_t b = c0 + min(b0 + u * kRowWaves, here - 1);          // behind the last block: that one again, for nobody
+                lo[u] = *reinterpret_cast<const i32x4*>(w + b * 128);
+                hi[u] = *reinterpret_cast<const i32x4*>(w + b * 128 + 16);
+                sw[u] = ws[b];
+            }
+        };
+        ahead(wave);
+        if (c0) __syncthreads();                                            // everyone is done with the last codes
+        for (uint32_t t = threadIdx.x >> 4; t < rows * here; t += 4 * kRowWaves) {
+            const uint32_t xr = t / here, b = t % here;
+            const uint64_t k = (uint64_t)(c0 + b) * 128 + 8 * r;
+            const int left = k < d.k ? (int)min((uint64_t)8, d.k - k) : 0;
+            Eight<T> v;
+            v.load((const T*)d.x + xr * d.ldx + (left ? k : 0), left);
+            const uint32_t byte = scale_byte(row_max_u32(v.amax()));
+            *reinterpret_cast<uint2*>(codes + xr * pitch + b * 128 + 8 * r) = coded(v.encode(scale_value(byte)), byte);
+            if (r == 0) bytes[xr * here + b] = (uint8_t)byte;
         }
+        __syncthreads();
+        const uint32_t xr = min((uint32_t)r, rows - 1);                     // rows behind the last: its results again, for nobody
+        for (uint32_t b0 = wave; b0 < here; b0 += kRowWaves * kRowBlocks) {
+            if (b0 != (uint32_t)wave) ahead(b0);
 #pragma unroll
-        for (int u = 0; u < kRowBlocks; ++u)
+            for (int u = 0; u < kRowBlocks; ++u) {
+                const uint32_t b = b0 + u * kRowWaves;
+                if (b >= here) break;
+                const i32x4 xl = *reinterpret_cast<const i32x4*>(codes + xr * pitch + b * 128 + q * 32), xh = *reinterpret_cast<const i32x4*>(codes + xr * pitch + b * 128 + q * 32 + 16);
+                const uint32_t sx = bytes[xr * here + b];
+                if constexpr (sizeof(T) == 4) {      // a 32-bit result: see EXACT above
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint64_t k = (uint64_t)(b0 + u * kRowWaves) * 128 + q * 32 + 8 * i;
-                const int left = there && k < d.k ? (int)min((uint64_t)8, d.k - k) : 0;
-                v[u][i].load(x + (left ? k : 0), left);
-            }
-#pragma unroll
-        for (int u = 0; u < kRowBlocks; ++u) {
-            uint32_t a = max(max(v[u][0].amax(), v[u][1].amax()), max(v[u][2].amax(), v[u][3].amax()));
-            a = max(a, (uint32_t)__shfl_xor((int)a, 16));
-            a = max(a, (uint32_t)__shfl_xor((int)a, 32));
-            const uint32_t sx = scale_byte(a);
-            const float scale = scale_value(sx);
-            i32x8 fx;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint2 c = coded(v[u][i].encode(scale), sx);
-                fx[2 * i] = (int)c.x;
-                fx[2 * i + 1] = (int)c.y;
-            }
-            if constexpr (sizeof(T) == 4) {      // a 32-bit result: see EXACT above
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const i32x4 part = i < 2 ? lo[u] : hi[u];
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(part[2 * (i & 1)], part[2 * (i & 1) + 1], scale_value(sw[u])),
-                                                                  widen8(fx[2 * i], fx[2 * i + 1], scale), acc, 0, 0, 0);
+                    for (int i = 0; i < 4; ++i) {
+                        const i32x4 pw = i < 2 ? lo[u] : hi[u], px = i < 2 ? xl : xh;
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(pw[2 * (i & 1)], pw[2 * (i & 1) + 1], scale_value(sw[u])),
+                                                                      widen8(px[2 * (i & 1)], px[2 * (i & 1) + 1], scale_value(sx)), acc, 0, 0, 0);
+                    }
+                } else {
+                    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(lo[u], hi[u], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                                           __builtin_shufflevector(xl, xh, 0, 1, 2, 3, 4, 5, 6, 7), acc, 0, 0, 0, sw[u], 0, (int)sx);
                 }
-            } else {
-                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(lo[u], hi[u], 0, 1, 2, 3, 4, 5, 6, 7), fx, acc, 0, 0, 0, sw[u], 0, (int)sx);
             }
         }
     }

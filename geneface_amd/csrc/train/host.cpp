@@ -12,11 +12,11 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
-#include <limits>
+#include <algorithm>
+#include <cstring>
 #include <optional>
 #include <stdexcept>
 #include <string>
-#include <unordered_set>
 #include <vector>
 
 #include "geneface_train_hip.h"
@@ -125,17 +125,25 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& m, const Te
     for (const Tensors* l : {&m, &v, &steps}) same_device(all, *l, dev);
     if (eight) { same_device(all, *m_scales, dev); same_device(all, *v_scales, dev); }
     const c10::OptionalDeviceGuard guard(dev);
-    std::unordered_set<const void*> seen[5];
+    std::vector<const void*> places[4];      // of steps, parameters, moments, scales: each to be given once
+    for (auto& p : places) p.reserve(2 * n);
     for (size_t i = 0; i < n; ++i) {
         const bool dense = params[i].is_contiguous() && m[i].is_contiguous() && v[i].is_contiguous() && (!eight || ((*m_scales)[i].is_contiguous() && (*v_scales)[i].is_contiguous()));
         refuse_unless(dense, "adamw_step: parameters and their state must be contiguous tensors");
         if (!grads[i].is_contiguous()) grads[i] = grads[i].contiguous();
-        bool first = seen[0].insert(steps[i].data_ptr()).second;
-        if (params[i].numel()) {      // (empty tensors have no address)
-            first = first && seen[1].insert(params[i].data_ptr()).second && seen[2].insert(m[i].data_ptr()).second && seen[2].insert(v[i].data_ptr()).second;
-            if (eight) first = first && seen[3].insert((*m_scales)[i].data_ptr()).second && seen[3].insert((*v_scales)[i].data_ptr()).second;
+        places[0].push_back(steps[i].data_ptr());
+        if (!params[i].numel()) continue;      // (empty tensors have no address)
+        places[1].push_back(params[i].data_ptr());
+        places[2].push_back(m[i].data_ptr());
+        places[2].push_back(v[i].data_ptr());
+        if (eight) {
+            places[3].push_back((*m_scales)[i].data_ptr());
+            places[3].push_back((*v_scales)[i].data_ptr());
         }
-        refuse_unless(first, "adamw_step: the same tensor is given twice");
+    }
+    for (auto& p : places) {
+        std::sort(p.begin(), p.end());
+        refuse_unless(std::adjacent_find(p.begin(), p.end()) == p.end(), "adamw_step: the same tensor is given twice");
     }
     gf_adamw_t d = {};
     d.state_bits = eight ? 8 : 32;

@@ -96,6 +96,9 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.last_grad_norm = state_bits, max_grad_norm, None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):      # torch's keeps only state and groups: copies and pickles need these as well
+        return {**super().__getstate__(), "state_bits": self.state_bits, "max_grad_norm": self.max_grad_norm, "last_grad_norm": None}
+
     def _keys(self):
         return ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if self.state_bits == 8 else ())
 

@@ -85,7 +85,8 @@ def test_a_block_with_no_number_is_none(bad):
 
 
 SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (5, 1111, 2050), (16, 128, 96), (17, 3, 1000), (33, 129, 148), (128, 128, 128), (129, 127, 255), (200, 300, 4000),
-          (1000, 129, 148), (4099, 128, 96), (300, 2, 128), (700, 900, 513), (3500, 4100, 130)]
+          (1000, 129, 148), (4099, 128, 96), (300, 2, 128), (700, 900, 513), (3500, 4100, 130),
+          (16, 40, 9000), (1, 33, 140000), (3, 20, 50000), (40, 30, 600), (40, 30, 700), (40, 300, 20000), (130, 257, 131), (260, 70, 90)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -108,6 +109,20 @@ def test_product_and_gradients(M, N, K, dtype):
     _near(y.detach(), xr @ wt.t(), xr.abs() @ wt.abs().t(), dtype, K, "y")
     _near(dx, gr @ wt, gr.abs() @ wt.abs(), dtype, N, "dx")
     _near(dw, gc.t() @ xc, gc.abs().t() @ xc.abs(), torch.float32, M, "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, N, K", [(110001, 128, 128), (110000, 5, 7), (110001, 1, 100), (100500, 101, 1)])
+def test_thin_layer_over_many_rows(M, N, K, dtype):
+    """More tiles of 128 rows than workgroups: each goes on to others.  Rows of whole numbers that e4m3 holds exactly, so sums are exact too."""
+    g = torch.Generator().manual_seed(M + N)
+    whole = lambda *s: torch.randint(-2, 3, s, generator=g).float()      # noqa: E731
+    x, w, dy = whole(M, K), whole(N, K), whole(M, N)
+    a, b = x.to(dtype).cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    y = fp8.linear(a, b)
+    dx, dw = torch.autograd.grad(y, (a, b), dy.to(dtype).cuda())
+    near = lambda got, want: torch.equal(got.float().cpu(), want.to(got.dtype).float())      # noqa: E731
+    assert near(y.detach(), x @ w.t()) and near(dx, dy @ w) and near(dw, dy.double().t() @ x.double())
 
 
 @pytest.mark.parametrize("tx, tw", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.float16), (torch.float16, torch.bfloat16)])

@@ -4,6 +4,7 @@ Tolerances are counts of roundings.  eps = 2^-24 is half a step of a 32-bit valu
 relative to |m| + |g|, 4 on the second relative to itself, 6 more on the quotient, 2 on the parameter, then one to the parameter's type.  The tests
 allow twice that.  An 8-bit code is floor(value / spacing + u): it can differ only where that sum is within the value's own error of a whole number.
 """
+import copy
 import math
 
 import pytest
@@ -299,6 +300,20 @@ def test_state_dict_continues_bit_for_bit(bits, tmp_path):
     steps(a, oa, (2, 3))
     steps(b, ob, (2, 3))
     assert all(torch.equal(x, y) for x, y in zip(a, b)) and ob.param_groups[0]["lr"] == 1e-2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copied_optimizer_continues(bits):
+    p = torch.nn.Parameter(torch.randn(300, generator=_gen(3)).cuda())
+    p.grad = torch.randn(300, generator=_gen(4)).cuda()
+    o = optim.AdamW([p], lr=1e-2, state_bits=bits, max_grad_norm=1.0)
+    o.step()
+    c = copy.deepcopy(o)
+    q = c.param_groups[0]["params"][0]
+    q.grad = p.grad.clone()
+    o.step()
+    c.step()
+    assert q is not p and c.state_bits == bits and torch.equal(p.detach(), q.detach())
 
 
 @pytest.mark.parametrize("bits", [32, 8])
