@@ -16,8 +16,8 @@ constexpr int kTensors = 56;              // per launch: 56 x 64 bytes + first w
 struct AdamwArgs {
     gf_adamw_tensor_t t[kTensors];
     uint32_t first[kTensors];             // first workgroup of each tensor, 0xffffffff behind the last
-    double beta1, beta2, lr;
-    float eps, weight_decay, max_norm;
+    double beta1, beta2, lr, weight_decay, max_norm;
+    float eps;
     uint32_t chunk;                       // values per workgroup, a multiple of 1024
     const float* lr_device;
     const float* grad_scale;
@@ -47,7 +47,7 @@ __device__ __forceinline__ Hyper hyper_of(const AdamwArgs& a, float t) {
     const double lr = a.lr_device ? (double)*a.lr_device : a.lr;
     const uint32_t ti = (uint32_t)t;
     Hyper h;
-    h.shrink = (float)(1.0 - lr * (double)a.weight_decay);
+    h.shrink = (float)(1.0 - lr * a.weight_decay);
     h.om_beta1 = (float)(1.0 - a.beta1);
     h.beta2 = (float)a.beta2;
     h.om_beta2 = (float)(1.0 - a.beta2);
@@ -56,7 +56,7 @@ __device__ __forceinline__ Hyper hyper_of(const AdamwArgs& a, float t) {
     h.eps = a.eps;
     double c = a.grad_scale ? 1.0 / (double)*a.grad_scale : 1.0;
     if (a.grad_norm) {
-        const double q = (double)a.max_norm / ((double)*a.grad_norm + 1e-6);
+        const double q = a.max_norm / ((double)*a.grad_norm + 1e-6);
         c *= q >= 1.0 ? 1.0 : q;          // a norm that is no number leaves none
     }
     h.grad = (float)c;
@@ -323,7 +323,7 @@ GF_EXPORT int gf_adamw_step(const gf_adamw_t* d, void* stream) {
 
     AdamwArgs a;
     a.beta1 = d->beta1; a.beta2 = d->beta2; a.lr = d->lr;
-    a.eps = (float)d->eps; a.weight_decay = (float)d->weight_decay; a.max_norm = (float)d->max_norm;
+    a.weight_decay = d->weight_decay; a.max_norm = d->max_norm; a.eps = (float)d->eps;
     a.chunk = chunk;
     a.count_steps = most <= chunk;
     a.lr_device = d->lr_device; a.grad_scale = d->grad_scale; a.found_inf = d->found_inf; a.grad_norm = d->grad_norm;

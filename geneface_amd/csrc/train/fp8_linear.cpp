@@ -75,6 +75,15 @@ static int size_error(const char* what, uint64_t m, uint64_t n, uint64_t k) {
     return GF_OK;
 }
 
+// gf_fp8_matmul adds up at most 65535 blocks: what the backward call would refuse is refused before there is anything to go back to.
+static int sum_error(const gf_fp8_linear_t& d) {
+    if (thin(d.n, d.k)) return GF_OK;
+    const uint64_t most = 65535ull * 128;
+    if (d.k > most || (d.keep_w && d.n > most) || (d.keep_x && d.m > most))
+        return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: more than %llu values along a sum", (unsigned long long)most);
+    return GF_OK;
+}
+
 }  // namespace gf
 
 using namespace gf;
@@ -82,6 +91,7 @@ using namespace gf;
 GF_EXPORT int gf_fp8_linear_plan(gf_fp8_linear_t* d) {
     if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear_plan: null descriptor");
     if (const int rc = size_error("gf_fp8_linear_plan", d->m, d->n, d->k)) return rc;
+    if (const int rc = sum_error(*d)) return rc;
     Pieces s{nullptr}, f{nullptr}, b{nullptr};
     saved_pieces(s, d->m, d->n, d->k, d->keep_w, d->keep_x);
     forward_pieces(f, *d);
@@ -95,6 +105,7 @@ GF_EXPORT int gf_fp8_linear_plan(gf_fp8_linear_t* d) {
 GF_EXPORT int gf_fp8_linear(const gf_fp8_linear_t* d, void* stream) {
     if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: null descriptor");
     if (const int rc = size_error("gf_fp8_linear", d->m, d->n, d->k)) return rc;
+    if (const int rc = sum_error(*d)) return rc;
     if (!d->x || !d->y || (!d->w && (!d->codes || !d->scales))) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: null pointer");
     if (!d->w && (d->keep_w || d->keep_x)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: a weight given as codes has no backward call");
     if (!d->w && d->m <= 16) {

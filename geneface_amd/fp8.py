@@ -127,7 +127,12 @@ def linear(x, weight):
     """x [..., K] times a weight's transpose, [..., N] in x's type (under autocast: in its type), both brought to 8 bits in blocks of 128.
 
     weight: a tensor [N, K], quantised in the call, with gradients to x and to the weight; or an Fp8Weight, without gradients.  x, weight: float32,
-    bfloat16 or float16, each its own; the gradients have their input's type."""
+    bfloat16 or float16, each its own; the gradients have their input's type.  At most 8388480 values along each sum, unless both of the weight's
+    sides are 128 or less.  Results of 16 bits are added up on the 8-bit matrix instructions (about 17 bits within one instruction, 32 between
+    them), results of 32 bits in 32.
+
+    Both directions may be captured into a graph.  As with any torch node, a backward pass is captured only while no graph of the same leaves lives
+    that was built outside the capture.  Gradients of the gradients are refused."""
     if isinstance(weight, Fp8Weight):
         return host().linear_packed(x, weight.values, weight.scales, weight.in_features)
     return host().linear(x, weight)

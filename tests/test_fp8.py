@@ -103,6 +103,11 @@ def test_the_library_refuses_bad_descriptors(hip_lib):
     f = lambda **k: fp8.GfFp8Linear(**{"x": 16, "ldx": 150, "w": 16, "ldw": 150, "m": 300, "n": 200, "k": 150, "y": 16, "workspace": 256, "saved": 256, "keep_x": 1, **k})      # noqa: E731
     refused(hip_lib.gf_fp8_linear_plan(None), b"null")
     refused(hip_lib.gf_fp8_linear_plan(C.byref(f(k=0))), b"empty")
+    for change in (dict(m=1 << 24), dict(k=1 << 24), dict(n=1 << 24, keep_w=1)):
+        refused(hip_lib.gf_fp8_linear_plan(C.byref(f(**change))), b"along a sum")
+        refused(hip_lib.gf_fp8_linear(C.byref(f(**change)), None), b"along a sum")
+    for change in (dict(m=1 << 24, keep_x=0), dict(n=1 << 24), dict(m=1 << 24, n=128, k=128)):
+        assert hip_lib.gf_fp8_linear_plan(C.byref(f(**change))) == 0
     p = f(keep_w=1)
     assert hip_lib.gf_fp8_linear_plan(C.byref(p)) == 0 and p.saved_bytes >= 150 * 256 + 4 + 150 * 384 + 3 * 150 and p.workspace_bytes >= 300 * 256 and p.backward_bytes >= 300 * 256 + 200 * 384
     refused(hip_lib.gf_fp8_linear(None, None), b"null")
