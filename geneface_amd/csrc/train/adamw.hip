@@ -23,6 +23,7 @@ struct AdamwArgs {
     const float* grad_scale;
     const float* found_inf;
     const float* grad_norm;
+    const double* grad_norm_wide;
     uint32_t count_steps;                 // 1: every tensor of the call has one workgroup, which counts its step itself
 };
 static_assert(sizeof(AdamwArgs) <= 4096, "kernel arguments");
@@ -56,15 +57,25 @@ __device__ __forceinline__ Hyper hyper_of(const AdamwArgs& a, float t) {
     h.eps = a.eps;
     double c = a.grad_scale ? 1.0 / (double)*a.grad_scale : 1.0;
     if (a.grad_norm) {
-        const double q = a.max_norm / ((double)*a.grad_norm + 1e-6);
+        double norm = *a.grad_norm;
+        if (a.grad_norm_wide && (float)*a.grad_norm_wide == *a.grad_norm) norm = *a.grad_norm_wide;      // (the 32-bit one as it was written)
+        const double q = a.max_norm / (norm + 1e-6);
         c *= q >= 1.0 ? 1.0 : q;          // a norm that is no number leaves none
     }
     h.grad = (float)c;
     return h;
 }
 
-__device__ __forceinline__ float moment1(const Hyper& h, float m, float g) { return m + h.om_beta1 * (g - m); }
-__device__ __forceinline__ float moment2(const Hyper& h, float v, float g) { return h.beta2 * v + h.om_beta2 * g * g; }
+// Every operation on the moments rounds by itself, as a formula written out in 32-bit operations does.  An 8-bit code is a step function of its
+// value: with the same roundings the state is the same bit for bit, however long two runs of the formula go side by side.
+__device__ __forceinline__ float moment1(const Hyper& h, float m, float g) {
+#pragma clang fp contract(off)
+    return m + h.om_beta1 * (g - m);
+}
+__device__ __forceinline__ float moment2(const Hyper& h, float v, float g) {
+#pragma clang fp contract(off)
+    return h.beta2 * v + h.om_beta2 * g * g;
+}
 __device__ __forceinline__ float updated(const Hyper& h, float p, float m, float r) { return p * h.shrink - h.rate * m / (r * h.inv_root + h.eps); }
 
 __device__ __forceinline__ uint32_t tensor_of(const AdamwArgs& a, uint32_t block) {
@@ -100,7 +111,7 @@ __device__ __forceinline__ void step32(const gf_adamw_tensor_t& t, const Hyper& 
 }
 
 // ---- 8-bit moments -------------------------------------------------------------------------------------------------------------------------
-// A block of 128 values has one 32-bit scale a / 448, a its largest magnitude (2^-100 at least, so that 448 / a is finite).  Sixteen lanes share a
+// A block of 128 values has one 32-bit scale a * (1 / 448), a its largest magnitude (2^-100 at least, so that its reciprocal is finite).  Sixteen lanes share a
 // block: lane j holds values 4j .. 4j+3 and 64+4j .. 64+4j+3, so that every load of a row of lanes is 256 consecutive bytes of 32-bit values.
 // Rounding to nearest would lose every change below half a spacing (up to 6 % of the value; the second moment moves by 1 - beta2 a step).  The
 // value is therefore rounded to floor(value / spacing + u) with u the fractional part of index phi_1 + step phi_2 (a two-dimensional Weyl
@@ -137,6 +148,17 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, uint32_t w, int left) 
     for (int i = 0; i < 4; ++i) if (i < left) dst[i] = (uint8_t)(w >> (8 * i));
 }
 
+// The square root to nearest from one to a unit in the last place: a neighbour is the nearer one where the residual of the middle says so.  (The
+// compiler's own also scales values below 2^-96, whose residual leaves the type's range; here those may be a unit off.  That scaling is half as
+// many operations again, and they are what this kernel has least room for: 506 us with it, 482 so, for 200 M values.)
+__device__ __forceinline__ float sqrt_nearest(float x) {
+    const float s = __builtin_amdgcn_sqrtf(x);
+    const float below = __uint_as_float(__float_as_uint(s) - 1), above = __uint_as_float(__float_as_uint(s) + 1);
+    const float down = __builtin_fmaf(-below, s, x), up = __builtin_fmaf(-above, s, x);
+    const float r = down <= 0.0f ? below : s;
+    return up > 0.0f ? above : r;
+}
+
 template <typename T>
 __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h, uint64_t begin, uint64_t end, uint32_t word) {
     T* p = (T*)t.p;
@@ -164,8 +186,8 @@ __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h
         for (int k = 0; k < 8; ++k) {      // (values that are not there are zeros and stay so)
             const float x = fg[k] * h.grad;
             fm[k] = moment1(h, fm[k], x);
-            // square root and reciprocal to one unit in the last place: correctly rounded ones cost as much again as all else here
-            fr[k] = __builtin_amdgcn_sqrtf(moment2(h, fr[k] * fr[k], x));
+            fr[k] = sqrt_nearest(moment2(h, fr[k] * fr[k], x));
+            // the reciprocal to one unit in the last place: nothing but this step's p depends on it
             fp[k] = fp[k] * h.shrink - h.rate * fm[k] * __builtin_amdgcn_rcpf(fr[k] * h.inv_root + h.eps);
             am = max_abs(am, fm[k]);
             ar = max_abs(ar, fr[k]);
@@ -173,7 +195,7 @@ __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h
         // as integers: what is no number stays the largest and makes the whole block none
         const uint32_t bm = row_max_u32(__float_as_uint(am)), br = row_max_u32(__float_as_uint(ar));
         const float a_m = max_abs(kTiny, __uint_as_float(bm)), a_r = max_abs(kTiny, __uint_as_float(br));
-        const float inv_m = 448.0f / a_m, inv_r = 448.0f / a_r;
+        const float inv_m = 1.0f / a_m * 448.0f, inv_r = 1.0f / a_r * 448.0f;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const uint32_t seed = (uint32_t)(i0 + 64 * q) * kDitherIndex + word;
@@ -192,7 +214,7 @@ __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h
                 store4_of(p + i, left[q], fp + 4 * q);
             }
         }
-        if (lane16 == 0) { t.m_scale[b] = a_m / 448.0f; t.v_scale[b] = a_r / 448.0f; }
+        if (lane16 == 0) { t.m_scale[b] = a_m * (1.0f / 448.0f); t.v_scale[b] = a_r * (1.0f / 448.0f); }
     }
 }
 
@@ -287,12 +309,15 @@ __global__ __launch_bounds__(kThreads) void k_norm(const NormArgs a) {
     if (threadIdx.x == 0) a.sums[blockIdx.x] = s;
 }
 
-__global__ __launch_bounds__(1024) void k_norm_finish(const double* sums, uint32_t count, const float* grad_scale, float* out) {
+__global__ __launch_bounds__(1024) void k_norm_finish(const double* sums, uint32_t count, const float* grad_scale, float* out, double* wide) {
     __shared__ double lds[16];
     double s = 0;
     for (uint32_t i = threadIdx.x; i < count; i += 1024) s += sums[i];
     s = block_sum(s, lds);
-    if (threadIdx.x == 0) *out = (float)(sqrt(s) / (grad_scale ? (double)*grad_scale : 1.0));
+    if (threadIdx.x) return;
+    const double norm = sqrt(s) * (grad_scale ? 1.0 / (double)*grad_scale : 1.0);
+    *out = (float)norm;
+    if (wide) *wide = norm;
 }
 
 }  // namespace gf
@@ -326,7 +351,7 @@ GF_EXPORT int gf_adamw_step(const gf_adamw_t* d, void* stream) {
     a.weight_decay = d->weight_decay; a.max_norm = d->max_norm; a.eps = (float)d->eps;
     a.chunk = chunk;
     a.count_steps = most <= chunk;
-    a.lr_device = d->lr_device; a.grad_scale = d->grad_scale; a.found_inf = d->found_inf; a.grad_norm = d->grad_norm;
+    a.lr_device = d->lr_device; a.grad_scale = d->grad_scale; a.found_inf = d->found_inf; a.grad_norm = d->grad_norm; a.grad_norm_wide = d->grad_norm_wide;
     const hipStream_t s = gf_stream(stream);
     for (uint32_t i = 0; i < d->count;) {
         uint32_t k = 0, blocks = 0;
@@ -387,6 +412,6 @@ GF_EXPORT int gf_grad_norm(const gf_grad_norm_t* d, void* stream) {
         k_norm<<<blocks, kThreads, 0, s>>>(a);
         done += blocks;
     }
-    k_norm_finish<<<1, 1024, 0, s>>>((const double*)d->workspace, done, d->grad_scale, d->norm_out);
+    k_norm_finish<<<1, 1024, 0, s>>>((const double*)d->workspace, done, d->grad_scale, d->norm_out, d->norm_out_wide);
     return gf_check_launch("gf_grad_norm");
 }

@@ -93,7 +93,8 @@ const float* scalar(const char* name, const std::optional<Tensor>& t, const at::
 
 void adamw_step(const Tensors& params, Tensors grads, const Tensors& m, const Tensors& v, const Tensors& steps, double lr, const std::optional<Tensor>& lr_device,
                 double beta1, double beta2, double eps, double weight_decay, const std::optional<Tensors>& m_scales, const std::optional<Tensors>& v_scales,
-                const std::optional<Tensor>& grad_scale, const std::optional<Tensor>& found_inf, const std::optional<Tensor>& grad_norm, double max_norm) {
+                const std::optional<Tensor>& grad_scale, const std::optional<Tensor>& found_inf, const std::optional<Tensor>& grad_norm, const std::optional<Tensor>& grad_norm_wide,
+                double max_norm) {
     const bool eight = m_scales.has_value();
     const size_t n = params.size();
     for (const Tensors* l : {(const Tensors*)&grads, &m, &v, &steps, eight ? &*m_scales : &m, eight ? &*v_scales : &v})
@@ -152,6 +153,8 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& m, const Te
     d.grad_scale = scalar("grad_scale", grad_scale, dev);
     d.found_inf = scalar("found_inf", found_inf, dev);
     d.grad_norm = scalar("grad_norm", grad_norm, dev);
+    if (grad_norm_wide && grad_norm_wide->device() == dev && grad_norm_wide->scalar_type() == at::kDouble && grad_norm_wide->numel() == 1)
+        d.grad_norm_wide = static_cast<const double*>(grad_norm_wide->data_ptr());
     std::vector<gf_adamw_tensor_t> table;
     table.reserve(n);
     for (int kind = 0; kind < 3; ++kind) {
@@ -174,7 +177,7 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& m, const Te
                 if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-Tensor grad_norm(Tensors grads, const std::optional<Tensor>& grad_scale) {
+std::pair<Tensor, Tensor> grad_norm(Tensors grads, const std::optional<Tensor>& grad_scale) {
     refuse_unless(!grads.empty(), "grad_norm: no gradients");
     strided("grad_norm", grads);
     const at::Device dev = grads[0].device();
@@ -189,9 +192,10 @@ Tensor grad_norm(Tensors grads, const std::optional<Tensor>& grad_scale) {
     }
     const Tensor out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
     const Tensor work = at::empty({(int64_t)api.grad_norm_workspace_bytes((uint32_t)table.size())}, at::TensorOptions().dtype(at::kByte).device(dev));
-    const gf_grad_norm_t d = {table.data(), (uint32_t)table.size(), 0, scalar("grad_scale", grad_scale, dev), (float*)out.data_ptr(), work.data_ptr()};
+    const Tensor wide = at::empty({}, at::TensorOptions().dtype(at::kDouble).device(dev));
+    const gf_grad_norm_t d = {table.data(), (uint32_t)table.size(), 0, scalar("grad_scale", grad_scale, dev), (float*)out.data_ptr(), work.data_ptr(), (double*)wide.data_ptr()};
     check(api.grad_norm(&d, stream_of(dev)));
-    return out;
+    return {out, wide};
 }
 
 // ---- 8-bit linear --------------------------------------------------------------------------------------------------------------------------

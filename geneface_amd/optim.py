@@ -4,7 +4,7 @@ What the reference's tasks build around the model (tasks/radnerfs/radnerf.py:53-
 kernels of this library: `AdamW` is a torch optimizer (param groups, state dict, GradScaler), `adamw_step` and `grad_norm` are the two calls below
 it.  With `weight_decay=0` it is Adam.
 
-8-bit moments: e4m3 codes with one 32-bit scale for each 128 consecutive values of a tensor, max(largest magnitude, 2^-100) / 448.  The second
+8-bit moments: e4m3 codes with one 32-bit scale for each 128 consecutive values of a tensor, max(largest magnitude, 2^-100) times 1 / 448.  The second
 moment is held as its square root, which halves the range it needs.  Codes are rounded by a dither that depends on the step and on the value's
 index only, so a step is reproducible and changes far below the format's spacing add up over the steps; a second moment above zero never becomes
 zero.  A block that meets a gradient that is no finite number is none afterwards (all 128 values).
@@ -29,20 +29,23 @@ class GfAdamw(C.Structure):
     """ctypes mirror of gf_adamw_t (include/geneface_train_hip.h)."""
     _fields_ = [("tensors_host", _vp), ("count", C.c_uint32), ("dtype", C.c_uint32), ("state_bits", C.c_uint32), ("_pad", C.c_uint32)] + \
                [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + \
-               [(n, _vp) for n in ("lr_device", "grad_scale", "found_inf", "grad_norm")]
+               [(n, _vp) for n in ("lr_device", "grad_scale", "found_inf", "grad_norm", "grad_norm_wide")]
 
 
 class GfGradNorm(C.Structure):
     """ctypes mirror of gf_grad_norm_t."""
-    _fields_ = [("tensors_host", _vp), ("count", C.c_uint32), ("_pad", C.c_uint32)] + [(n, _vp) for n in ("grad_scale", "norm_out", "workspace")]
+    _fields_ = [("tensors_host", _vp), ("count", C.c_uint32), ("_pad", C.c_uint32)] + [(n, _vp) for n in ("grad_scale", "norm_out", "workspace", "norm_out_wide")]
 
 
 def grad_norm(grads, grad_scale=None):
     """sqrt(sum of the squares of all `grads`) / grad_scale as a float32 tensor without dimensions, added up in 64 bits in a fixed order.
 
     grads: tensors of float32, bfloat16 or float16 on one device (None entries are left out).  grad_scale: one float32 on that device, the
-    factor the gradients carry (GradScaler's scale).  Infinities and NaN among the gradients give an infinite norm or NaN."""
-    return host().grad_norm([g for g in grads if g is not None], grad_scale)
+    factor the gradients carry (GradScaler's scale).  Infinities and NaN among the gradients give an infinite norm or NaN.  The
+    tensor's attribute `wide` holds the same in float64: `adamw_step` goes by it as long as it rounds to the tensor's own value."""
+    norm, wide = host().grad_norm([g for g in grads if g is not None], grad_scale)
+    norm.wide = wide
+    return norm
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, exp_avg_scales=None,
@@ -67,7 +70,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     if torch.is_tensor(lr) and lr.is_cuda:
         lr, lr_device = 0.0, lr
     host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, float(lr), lr_device, beta1, beta2, float(eps), float(weight_decay), exp_avg_scales,
-                      exp_avg_sq_scales, grad_scale, found_inf, grad_norm, math.inf if max_norm is None else float(max_norm))
+                      exp_avg_sq_scales, grad_scale, found_inf, grad_norm, getattr(grad_norm, "wide", None), math.inf if max_norm is None else float(max_norm))
 
 
 class AdamW(torch.optim.Optimizer):

@@ -33,7 +33,8 @@ typedef struct {
 } gf_adamw_tensor_t;
 
 /* Host descriptor; tensors_host is read during the call.  grad_scale, found_inf, grad_norm and lr_device are one float on the device each, or
- * NULL.  The gradients that enter are g / grad_scale min(1, max_norm / (grad_norm + 1e-6)).  Where *found_inf is not 0 nothing is changed, the
+ * NULL.  The gradients that enter are g / grad_scale min(1, max_norm / (grad_norm + 1e-6)); grad_norm_wide:
+ * the norm in 64 bits, taken where it rounds to *grad_norm, or NULL.  Where *found_inf is not 0 nothing is changed, the
  * step counts included.  lr_device replaces lr.  dtype: of p and g.  state_bits: 32 or 8. */
 typedef struct {
     const gf_adamw_tensor_t* tensors_host;
@@ -46,6 +47,7 @@ typedef struct {
     const float* grad_scale;
     const float* found_inf;
     const float* grad_norm;
+    const double* grad_norm_wide;
 } gf_adamw_t;
 
 /* p <- p (1 - lr wd);  m <- m + (1 - beta1)(g - m);  v <- beta2 v + (1 - beta2) g^2;
@@ -69,6 +71,7 @@ typedef struct {
     const float* grad_scale;
     float* norm_out;
     void* workspace;
+    double* norm_out_wide;      /* the same in 64 bits, or NULL */
 } gf_grad_norm_t;
 
 uint64_t gf_grad_norm_workspace_bytes(uint32_t count);

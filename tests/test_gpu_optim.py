@@ -389,6 +389,60 @@ def test_the_same_tensor_twice_is_refused():
     assert all(float(x.abs().max()) == 0 for x in a)
 
 
+def _written_out(q, scale, n):
+    return q.float().cpu() * scale.cpu().repeat_interleave(128)[:n]
+
+
+def _held(x, u, positive):
+    """Codes and scales of the moment x in single 32-bit operations (sums with the dither in 64 bits, where they are exact)."""
+    n = x.numel()
+    a = torch.nn.functional.pad(x.abs(), (0, -n % 128)).view(-1, 128).amax(1).clamp(min=2.0 ** -100)
+    y = (x * (a.reciprocal() * 448.0).repeat_interleave(128)[:n]).clamp(-448, 448)
+    gap = 2.0 ** ((torch.frexp(y)[1].double() - 1).clamp(min=-6) - 3)
+    k = torch.floor(y.abs().double() / gap + u)
+    if positive:
+        k = torch.where(x > 0, k.clamp(min=1), k)
+    return torch.copysign((k * gap).clamp(max=448).float(), y), a * torch.tensor(1.0 / 448.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_8_bit_state_is_the_formula_written_out_bit_for_bit(dtype):
+    """No tolerance: every operation of the moments rounds as the formula's own does, so after any number of steps the codes are its codes."""
+    b1, b2, scale = 0.9, 0.99, 1024.0
+    one = lambda x: torch.tensor(x, dtype=torch.float32)      # noqa: E731
+    n, g = 70001, _gen(77)
+    p = (0.3 * torch.randn(n, generator=g)).to(dtype).cuda()
+    m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+    ms, vs = (torch.zeros(-(-n // 128), device="cuda") for _ in range(2))
+    step, loss_scale = torch.zeros((), device="cuda"), torch.full((), scale, device="cuda")
+    for t in range(1, 9):
+        grad = (torch.randn(n, generator=g) * 2.0 ** torch.randint(-9, 5, (n,), generator=g) * (torch.rand(n, generator=g) > 0.3)).to(dtype)
+        m0, r0 = _written_out(m, ms, n), _written_out(v, vs, n)
+        norm = optim.grad_norm([grad.cuda()], grad_scale=loss_scale)
+        wide = float(norm.wide)
+        assert wide == pytest.approx(math.sqrt(float(grad.double().pow(2).sum())) / scale, rel=1e-13) and float(norm) == float(one(wide))
+        optim.adamw_step([p], [grad.cuda()], [m], [v], [step], lr=1e-3, betas=(b1, b2), exp_avg_scales=[ms], exp_avg_sq_scales=[vs], grad_scale=loss_scale,
+                         grad_norm=norm, max_norm=0.01)
+        x = grad.float() * one(min(1.0, 0.01 / (wide + 1e-6)) / scale)
+        u = ((torch.arange(n) * A + t * B) % 2 ** 32 // 4096).double() / 2 ** 20
+        # (torch's float32 square root on the CPU is a unit off for one value in 170; by way of 64 bits it is the nearest)
+        for value, q, s, shift in ((m0 + one(1 - b1) * (x - m0), m, ms, 0.0), ((one(b2) * (r0 * r0) + one(1 - b2) * x * x).double().sqrt().float(), v, vs, 0.5)):
+            code, held = _held(value, (u + shift) % 1, shift > 0)
+            assert torch.equal(s.cpu(), held), t
+            assert torch.equal(q.float().cpu(), code), t
+
+
+def test_a_norm_changed_by_the_caller_is_the_one_that_counts():
+    grad = torch.full((1000,), 1.0, device="cuda")
+    moved = []
+    for change in (lambda x: x, lambda x: x.mul_(4.0), lambda x: x.clone() * 4.0, lambda x: torch.full_like(x, 4.0 * float(x))):
+        p, m, v = (torch.zeros(1000, device="cuda") for _ in range(3))
+        norm = change(optim.grad_norm([grad]))
+        optim.adamw_step([p], [grad], [m], [v], [torch.zeros((), device="cuda")], lr=0.1, betas=(0.5, 0.5), eps=1.0, grad_norm=norm, max_norm=1.0)
+        moved.append(float(m[0]))
+    assert moved[0] == pytest.approx(0.5 / math.sqrt(1000), rel=1e-6) and all(x == pytest.approx(moved[0] / 4, rel=1e-6) for x in moved[1:])
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1.0, 1e30])
 def test_norm_over_mixed_types(scale):
     g = _gen(41)
