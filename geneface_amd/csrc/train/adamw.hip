@@ -344,7 +344,7 @@ GF_EXPORT int gf_adamw_step(const gf_adamw_t* d, void* stream) {
     // scalars (two powers in 64 bits, about half a microsecond) where there is more.
     uint32_t chunk = 1024;
     while (chunk < 8192 && total / chunk > 4096) chunk *= 2;
-    while (total / chunk > (1ull << 30)) chunk *= 2;
+    while (total / chunk > (1ull << 23)) chunk *= 2;      // a launch's work-items lie below 2^32
 
     AdamwArgs a;
     a.beta1 = d->beta1; a.beta2 = d->beta2; a.lr = d->lr;

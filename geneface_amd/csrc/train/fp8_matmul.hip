@@ -287,7 +287,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d) 
     __shared__ __align__(16) uint8_t codes[kRowBytes + 16 * 16];
     __shared__ uint8_t bytes[kRowBytes / 128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    const uint64_t n0 = (uint64_t)blockIdx.x * 16;
+    const uint64_t n0 = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16;
+    if (n0 >= d.n) return;
     const uint32_t blocks = (uint32_t)((d.k + 127) / 128), rows = (uint32_t)d.m;
     const uint64_t row = min(n0 + r, d.n - 1);
     const uint8_t* w = d.codes + row * blocks * 128 + q * 32;
@@ -354,32 +355,43 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d) 
     if (m < d.m && n < d.n) ((T*)d.out)[m * d.n + n] = (T)s;
 }
 
-// The tile's edge and how many ways the sum over K is split.  Tiles of 256 x 256 read half the bytes from LDS and L2 per product that those of
-// 128 x 128 do and are taken where there are enough of them to give every CU one and they reach little further behind the last row and column;
-// otherwise 128, of which two fit a CU, and the sum is split until
-// every CU has work, with at least four blocks of 128 in each split.
-struct Plan { uint32_t edge, tiles_m, tiles_n, splits, per_split; };
+// The tile and how many ways the sum over K is split: the choice with the least time of its longest CU, in units of 0.11 us.  A workgroup's step over
+// one block takes 2 of them for a tile of 64 x 64, 3 for 128 x 64, 5 for 128 x 128 and 17 for 256 x 256 (about 1.7 times that each for the 32-bit
+// result): large tiles read less per product, small ones give every CU one (the three small tiles all read some 32 bytes a clock and CU, which is what
+// bounds them; fragments straight from memory to registers, without LDS, read half of that).  A split's parts cost 45, their launch among it, and the way to memory and
+// back.  Measured, us, 64 x 64 / 128 x 64 / 128 x 128 / 256 x 256: m 333, n 2048, k 8192 16.9 / 21 / 22 / -, split in two 128 x 64 18.3, in four
+// 128 x 128 18.1; 512, 4096, 4096 16.6 / 13.7 / 17.1 / -; 2048 each 17.7 / 15.9 / 13.8 / 25.5; 4096 each 111 / 103 / 70 / 62.
+struct Plan { uint32_t edge_m, edge_n, tiles_m, tiles_n, splits, per_split; };
 
 static Plan plan_of(uint64_t m, uint64_t n, uint64_t blocks) {
-    Plan p;
-    auto tiles = [&](uint64_t edge) { return ((m + edge - 1) / edge) * ((n + edge - 1) / edge); };
-    p.edge = tiles(256) >= 192 && 4 * tiles(256) <= tiles(128) + tiles(128) / 8 ? 256 : 128;
-    p.tiles_m = (uint32_t)((m + p.edge - 1) / p.edge);
-    p.tiles_n = (uint32_t)((n + p.edge - 1) / p.edge);
-    const uint64_t t = tiles(p.edge);
-    uint64_t s = t >= 256 || p.edge == 256 ? 1 : 256 / t;
-    if (s > blocks / 4) s = blocks / 4;
-    if (s < 1) s = 1;
-    p.per_split = (uint32_t)((blocks + s - 1) / s);
-    p.splits = (uint32_t)((blocks + p.per_split - 1) / p.per_split);      // none of them empty
-    return p;
+    struct Kind { uint32_t edge_m, edge_n, units; };
+    constexpr Kind kinds[] = {{64, 64, 2}, {128, 64, 3}, {128, 128, 5}, {256, 256, 17}};
+    constexpr uint64_t kCus = 256;
+    Plan best = {};
+    double least = 0;
+    for (const Kind& k : kinds) {
+        Plan p = {k.edge_m, k.edge_n, (uint32_t)((m + k.edge_m - 1) / k.edge_m), (uint32_t)((n + k.edge_n - 1) / k.edge_n), 1, (uint32_t)blocks};
+        const uint64_t t = (uint64_t)p.tiles_m * p.tiles_n;
+        for (uint64_t want = 1;; want = kCus / t < blocks / 4 ? kCus / t : blocks / 4) {      // at least four blocks in each
+            p.per_split = (uint32_t)((blocks + want - 1) / want);
+            p.splits = (uint32_t)((blocks + p.per_split - 1) / p.per_split);                  // none of them empty
+            const double cost = (double)((t * p.splits + kCus - 1) / kCus) * p.per_split * k.units + (p.splits > 1 ? 45 + 1.8e-5 * (double)(m * n) * p.splits : 0);
+            if (!best.edge_m || cost < least) { best = p; least = cost; }
+            if (want > 1 || kCus / t < 2 || blocks < 8) break;
+        }
+    }
+    return best;
 }
 
 template <typename T, bool EXACT>
 static void launch_tiles(const MatmulArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid(p.tiles_m * p.tiles_n, p.splits);
-    if (p.edge == 256) k_matmul<T, EXACT, 4, 4, 2><<<grid, 256, 0, s>>>(a);
-    else k_matmul<T, EXACT, 2, 2, 4><<<grid, 256, 0, s>>>(a);
+    if (p.edge_m == 256) k_matmul<T, EXACT, 4, 4, 2><<<grid, 256, 0, s>>>(a);
+    else if (p.edge_n == 64 && p.edge_m == 64) k_matmul<T, EXACT, 1, 1, 4><<<grid, 256, 0, s>>>(a);
+    else if (p.edge_n == 64) k_matmul<T, EXACT, 2, 1, 4><<<grid, 256, 0, s>>>(a);
+    // four blocks under way where a CU has one workgroup (2048 each: 13.8 us, with two blocks 15.0), two where it has more (2500 each: 22.0, with four 26.5)
+    else if (grid.x * grid.y <= 256) k_matmul<T, EXACT, 2, 2, 4><<<grid, 256, 0, s>>>(a);
+    else k_matmul<T, EXACT, 2, 2, 2><<<grid, 256, 0, s>>>(a);
 }
 
 template <typename T>
@@ -401,8 +413,8 @@ static const char* operand_error(const gf_fp8_operand_t& o, uint64_t rows) {
     return nullptr;
 }
 
-static bool too_large(uint64_t m, uint64_t n, uint64_t blocks) {      // blocks: a tile's rows have to lie within 4 GB
-    return m >> 31 || n >> 31 || blocks > 65535 || ((m + 127) / 128) * ((n + 127) / 128) >> 31 || (m * n) >> 41;
+static bool too_large(uint64_t m, uint64_t n, uint64_t blocks) {      // blocks: a tile's rows have to lie within 4 GB; tiles: a launch's work-items below 2^32
+    return m >> 31 || n >> 31 || blocks > 65535 || ((m + 127) / 128) * ((n + 127) / 128) >> 22;
 }
 
 }  // namespace gf
@@ -449,7 +461,8 @@ GF_EXPORT int gf_fp8_rows(const gf_fp8_rows_t* d, void* stream) {
     if (d->k >> 31) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: matrix too large");
     if ((uintptr_t)d->codes % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: codes must start at a multiple of 16 bytes");
     if ((d->n + 15) / 16 >> 31) return gf_set_error(GF_ERR_INVALID, "gf_fp8_rows: matrix too large");
-    const uint32_t grid = (uint32_t)((d->n + 15) / 16);
+    const uint32_t groups = (uint32_t)((d->n + 15) / 16), wide = 1u << 20;      // a launch's work-items along x lie below 2^32
+    const dim3 grid(groups < wide ? groups : wide, (groups + wide - 1) / wide);
     const hipStream_t s = gf_stream(stream);
     if (d->dtype == F32) k_rows<float><<<grid, 64 * kRowWaves, 0, s>>>(*d);
     else if (d->dtype == BF16) k_rows<__bf16><<<grid, 64 * kRowWaves, 0, s>>>(*d);

@@ -17,7 +17,8 @@ __global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, con
     __shared__ uint32_t most[4][kTile];                                // a wave's largest magnitudes by column
     __shared__ __align__(16) uint8_t turned[kTile * kTile];
     const int t = threadIdx.x, j = t & 15, g = t >> 4, wave = t >> 6;  // columns 8j..8j+7 of the tile, rows 8g..8g+7
-    const uint32_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
+    const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, br = at / blocks_c, bc = at % blocks_c;      // behind the last: rows that are not there
+    if (br >= blocks_r) return;
     const uint64_t r0 = (uint64_t)br * kTile + 8 * g, c0 = (uint64_t)bc * kTile + 8 * j;
     const bool by_tile = d.tiles != 0;
 
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, con
 template <typename T>
 __global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d, const uint32_t blocks_c) {
     const int j = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const uint32_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
+    const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, br = at / blocks_c, bc = at % blocks_c;      // behind the last: rows that are not there
     const uint64_t r0 = (uint64_t)br * 32 + 2 * g, c0 = (uint64_t)bc * kTile + 8 * j;
     Eight<T> x[2];
     const int left = c0 < d.cols ? (int)min((uint64_t)8, d.cols - c0) : 0;
@@ -116,8 +117,9 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d
 
 template <typename T>
 static void launch_quantize(const gf_fp8_quantize_t& d, uint64_t rb, uint64_t cb, hipStream_t s) {
-    if (!d.col_codes && !d.tiles) k_quantize_rows<T><<<(uint32_t)((d.rows + 31) / 32 * cb), 256, 0, s>>>(d, (uint32_t)cb);
-    else k_quantize<T><<<(uint32_t)(rb * cb), 256, 0, s>>>(d, (uint32_t)rb, (uint32_t)cb);
+    auto grid = [](uint64_t n) { const uint64_t wide = 1u << 22; return dim3((uint32_t)(n < wide ? n : wide), (uint32_t)((n + wide - 1) / wide)); };      // work-items along x lie below 2^32
+    if (!d.col_codes && !d.tiles) k_quantize_rows<T><<<grid((d.rows + 31) / 32 * cb), 256, 0, s>>>(d, (uint32_t)cb);
+    else k_quantize<T><<<grid(rb * cb), 256, 0, s>>>(d, (uint32_t)rb, (uint32_t)cb);
 }
 
 }  // namespace gf
