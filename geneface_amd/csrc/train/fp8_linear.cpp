@@ -1,6 +1,7 @@
 // gf_fp8_linear and gf_fp8_linear_backward: a layer's products with what they need around them, as one call each.  Host code over the entry points of
 // fp8_quantize.hip and fp8_matmul.hip; what it decides is where everything lies in the caller's two buffers.
 #include "../common.hpp"
+#include "fp8_two.hpp"
 #include "geneface_train_hip.h"
 
 namespace gf {
@@ -118,20 +119,16 @@ GF_EXPORT int gf_fp8_linear(const gf_fp8_linear_t* d, void* stream) {
     const Saved s = saved_pieces(ps, d->m, d->n, d->k, d->keep_w, d->keep_x);
     const Forward f = forward_pieces(pf, *d);
     const uint64_t kb = blocks_of(d->k);
-    const uint8_t *w_codes = d->codes, *w_scales = d->scales;
-    if (d->w) {
-        uint8_t* tiles = d->keep_w ? s.w_scales : f.w_scales;
-        const gf_fp8_quantize_t q = {d->w, d->n, d->k, d->ldw, d->w_dtype, 1, f.w_codes, nullptr, s.w_codes, nullptr, tiles, 0, 0};
-        if (const int rc = gf_fp8_quantize(&q, stream)) return rc;
-        w_codes = f.w_codes;
-        w_scales = tiles;
-    }
+    const uint8_t *w_codes = d->w ? f.w_codes : d->codes, *w_scales = d->w ? (d->keep_w ? s.w_scales : f.w_scales) : d->scales;
+    const gf_fp8_quantize_t qw = {d->w, d->n, d->k, d->ldw, d->w_dtype, 1, f.w_codes, nullptr, s.w_codes, nullptr, d->keep_w ? s.w_scales : f.w_scales, 0, 0};
+    const gf_fp8_quantize_t qx = {d->x, d->m, d->k, d->ldx, d->dtype, 0, f.x_codes, f.x_scales, s.x_codes, s.x_scales, nullptr, d->m, d->k};
     if (thin(d->n, d->k)) {
+        if (d->w)
+            if (const int rc = gf_fp8_quantize(&qw, stream)) return rc;
         const gf_fp8_thin_t t = {d->x, d->ldx, d->m, d->n, d->k, w_codes, w_scales, d->y, s.x_codes, s.x_scales, d->dtype, 0};
         return gf_fp8_thin(&t, stream);
     }
-    const gf_fp8_quantize_t q = {d->x, d->m, d->k, d->ldx, d->dtype, 0, f.x_codes, f.x_scales, s.x_codes, s.x_scales, nullptr, d->m, d->k};
-    if (const int rc = gf_fp8_quantize(&q, stream)) return rc;
+    if (const int rc = d->w ? quantize_two(qw, qx, stream) : gf_fp8_quantize(&qx, stream)) return rc;
     const gf_fp8_matmul_t p = {{f.x_codes, f.x_scales, d->m, 0, 0}, {w_codes, w_scales, 0, kb, 1}, d->m, d->n, kb, d->y, d->dtype, 0, f.parts};
     return gf_fp8_matmul(&p, stream);
 }
@@ -153,13 +150,9 @@ GF_EXPORT int gf_fp8_linear_backward(const gf_fp8_linear_backward_t* d, void* st
     }
     const gf_fp8_quantize_t q = {d->dy, d->m, d->n, d->lddy, d->dtype, 0, b.row_codes, b.row_scales, b.col_codes, b.col_scales, nullptr, d->m, d->n};
     if (const int rc = gf_fp8_quantize(&q, stream)) return rc;
-    if (d->dx) {      // b is w by columns: its scales are those of the tiles, transposed
-        const gf_fp8_matmul_t p = {{b.row_codes, b.row_scales, d->m, 0, 0}, {s.w_codes, s.w_scales, 0, 1, blocks_of(d->k)}, d->m, d->k, blocks_of(d->n), d->dx, d->dtype, 0, b.parts};
-        if (const int rc = gf_fp8_matmul(&p, stream)) return rc;
-    }
-    if (d->dw) {
-        const gf_fp8_matmul_t p = {{b.col_codes, b.col_scales, d->n, 0, 0}, {s.x_codes, s.x_scales, d->k, 0, 0}, d->n, d->k, blocks_of(d->m), d->dw, d->w_dtype, 0, b.parts};
-        return gf_fp8_matmul(&p, stream);
-    }
-    return GF_OK;
+    // dx: b is w by columns, its scales those of the tiles, transposed
+    const gf_fp8_matmul_t x = {{b.row_codes, b.row_scales, d->m, 0, 0}, {s.w_codes, s.w_scales, 0, 1, blocks_of(d->k)}, d->m, d->k, blocks_of(d->n), d->dx, d->dtype, 0, b.parts};
+    const gf_fp8_matmul_t w = {{b.col_codes, b.col_scales, d->n, 0, 0}, {s.x_codes, s.x_scales, d->k, 0, 0}, d->n, d->k, blocks_of(d->m), d->dw, d->w_dtype, 0, b.parts};
+    if (d->dx && d->dw) return matmul_two(x, w, stream);
+    return gf_fp8_matmul(d->dx ? &x : &w, stream);
 }

@@ -6,6 +6,7 @@
 #include "../common.hpp"
 #include "fp8.hpp"
 #include "fp8_join.hpp"
+#include "fp8_two.hpp"
 #include "geneface_train_hip.h"
 #include <type_traits>
 #include <utility>
@@ -60,7 +61,7 @@ constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 
 // 5.6e-5 for log-normal ones, against 1e-7 of the bfloat16 instruction).  That is below half a step of a 16-bit result (2^-9, 2^-12), and not what a
 // 32-bit one should carry: for those the codes are widened to bfloat16 on the way out of LDS.
 template <typename T, bool EXACT, int TM, int TN, int STAGES>
-__device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
+__device__ __forceinline__ void matmul_tile(const MatmulArgs& d, const uint32_t block, const uint32_t split) {
     constexpr int BM = 64 * TM, BN = 64 * TN, LA = BM / 32, LB = BN / 32;      // 32 rows of 128 bytes a load of the workgroup
     auto stage_a = [](auto j) __attribute__((always_inline)) { return lds_array<BM * 128, decltype(j)::value>(); };
     auto stage_b = [](auto j) __attribute__((always_inline)) { return lds_array<BN * 128, 16 + decltype(j)::value>(); };
@@ -70,14 +71,14 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
     // workgroups read at one time is a few rows and columns of tiles, in its own L2.
     uint32_t tile_m, tile_n;
     {
-        const uint32_t total = d.tiles_m * d.tiles_n, xcd = blockIdx.x & 7, full = total / 8, rest = total % 8;
-        const uint32_t t = xcd * full + min(xcd, rest) + (blockIdx.x >> 3), band = t / (8 * d.tiles_n), in = t % (8 * d.tiles_n);
+        const uint32_t total = d.tiles_m * d.tiles_n, xcd = block & 7, full = total / 8, rest = total % 8;
+        const uint32_t t = xcd * full + min(xcd, rest) + (block >> 3), band = t / (8 * d.tiles_n), in = t % (8 * d.tiles_n);
         const uint32_t high = min(8u, d.tiles_m - band * 8);
         tile_m = __builtin_amdgcn_readfirstlane(band * 8 + in % high);
         tile_n = __builtin_amdgcn_readfirstlane(in / high);
     }
     const uint64_t m0 = (uint64_t)tile_m * BM, n0 = (uint64_t)tile_n * BN;
-    const uint32_t kb0 = blockIdx.y * d.per_split, nb = min(d.blocks, kb0 + d.per_split) - kb0, width = d.blocks * 128;
+    const uint32_t kb0 = split * d.per_split, nb = min(d.blocks, kb0 + d.per_split) - kb0, width = d.blocks * 128;
 
     auto buffer = [&](const uint8_t* codes, uint64_t row0, uint32_t rows, uint32_t tile) {
         const uint64_t have = (uint64_t)min(tile, rows - (uint32_t)row0) * width - (uint64_t)kb0 * 128;
@@ -239,7 +240,7 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
     constexpr int COLS = 32 * TN, PITCH = COLS * (int)sizeof(T) + 16, EACH = 16 / (int)sizeof(T), PIECES = COLS / EACH;
     static_assert(32 * PITCH <= BN * 128 && 32 * PITCH <= BM * 128, "staging");
     uint8_t* mine = wave == 0 ? stage_a(Const<0>{}) : wave == 1 ? stage_a(Const<1>{}) : wave == 2 ? stage_b(Const<0>{}) : stage_b(Const<1>{});
-    T* out = (T*)d.out + (uint64_t)blockIdx.y * d.m * d.n;
+    T* out = (T*)d.out + (uint64_t)split * d.m * d.n;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -272,7 +273,17 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d) {
 }
 
 template <typename T, bool EXACT, int TM, int TN, int STAGES>
-__global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN, STAGES>(d); }
+__global__ __launch_bounds__(256) void k_matmul(const MatmulArgs d) { matmul_tile<T, EXACT, TM, TN, STAGES>(d, blockIdx.x, blockIdx.y); }
+
+// Two products of small tiles and sums that are not split; the second one's begin at a multiple of 8, for the XCDs.
+template <typename A, typename B>
+__global__ __launch_bounds__(256) void k_matmul_two(const MatmulArgs a, const MatmulArgs b) {
+#ifdef __HIP_DEVICE_COMPILE__      // (the host's pass finds no candidate for these calls, and has no use for them)
+    const uint32_t tiles = a.tiles_m * a.tiles_n, first = (tiles + 7) & ~7u;
+    if (blockIdx.x >= first) matmul_tile<B, sizeof(B) == 4, 1, 1, 4>(b, blockIdx.x - first, 0);
+    else if (blockIdx.x < tiles) matmul_tile<A, sizeof(A) == 4, 1, 1, 4>(a, blockIdx.x, 0);
+#endif
+}
 
 // ---- a few rows ----------------------------------------------------------------------------------------------------------------------------
 // The weight's bytes bound it, and at the sizes it is called with, how many of them are under way at once and how long the way to the first product is.
@@ -417,6 +428,61 @@ static bool too_large(uint64_t m, uint64_t n, uint64_t blocks) {      // blocks:
     return m >> 31 || n >> 31 || blocks > 65535 || ((m + 127) / 128) * ((n + 127) / 128) >> 22;
 }
 
+static int matmul_error(const gf_fp8_matmul_t& d) {
+    if (!d.out) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null output");
+    if (d.dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: unknown dtype %u", d.dtype);
+    if (d.blocks == 0) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: no blocks to add up");
+    if (const char* e = operand_error(d.a, d.m)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: a: %s", e);
+    if (const char* e = operand_error(d.b, d.n)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: b: %s", e);
+    if (too_large(d.m, d.n, d.blocks)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: matrix too large (at most 65535 blocks along the sum)");
+    if (plan_of(d.m, d.n, d.blocks).splits > 1 && (!d.workspace || (uintptr_t)d.workspace % 16))
+        return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null or unaligned workspace");
+    return GF_OK;
+}
+
+static MatmulArgs args_of(const gf_fp8_matmul_t& d, const Plan& p) {
+    MatmulArgs a;
+    a.a = {d.a.codes, d.a.scales, d.a.pitch, d.a.stride_row, d.a.stride_block};
+    a.b = {d.b.codes, d.b.scales, d.b.pitch, d.b.stride_row, d.b.stride_block};
+    a.m = (uint32_t)d.m; a.n = (uint32_t)d.n; a.blocks = (uint32_t)d.blocks;
+    a.per_split = p.per_split; a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n;
+    a.out = d.out;
+    return a;
+}
+
+// f(T()) with the type that dtype names
+template <typename F>
+static void with_type(uint32_t dtype, F f) {
+    if (dtype == F32) f(float());
+    else if (dtype == BF16) f(__bf16());
+    else f(_Float16());
+}
+
+static void launch(const gf_fp8_matmul_t& d, hipStream_t s) {
+    const Plan p = plan_of(d.m, d.n, d.blocks);
+    with_type(d.dtype, [&](auto t) { launch_matmul<decltype(t)>(args_of(d, p), p, d.workspace, s); });
+}
+
+template <typename A, typename B>
+static void launch_matmul_two(const MatmulArgs& a, const MatmulArgs& b, uint32_t grid, hipStream_t s) { k_matmul_two<A, B><<<grid, 256, 0, s>>>(a, b); }
+
+int matmul_two(const gf_fp8_matmul_t& a, const gf_fp8_matmul_t& b, void* stream) {
+    if (const int rc = matmul_error(a)) return rc;
+    if (const int rc = matmul_error(b)) return rc;
+    const hipStream_t s = gf_stream(stream);
+    const Plan p = plan_of(a.m, a.n, a.blocks), q = plan_of(b.m, b.n, b.blocks);
+    const uint64_t ta = (uint64_t)p.tiles_m * p.tiles_n, tb = (uint64_t)q.tiles_m * q.tiles_n;
+    if (p.edge_m == 64 && q.edge_m == 64 && p.splits == 1 && q.splits == 1 && ta + tb < 1u << 22) {
+        with_type(a.dtype, [&](auto x) {
+            with_type(b.dtype, [&](auto y) { launch_matmul_two<decltype(x), decltype(y)>(args_of(a, p), args_of(b, q), (uint32_t)((ta + 7) / 8 * 8 + tb), s); });
+        });
+    } else {
+        launch(a, s);
+        launch(b, s);      // (their parts may lie in one workspace: the first product's are read before the second's are written)
+    }
+    return gf_check_launch("gf_fp8_matmul");
+}
+
 }  // namespace gf
 
 using namespace gf;
@@ -430,24 +496,8 @@ GF_EXPORT uint64_t gf_fp8_matmul_workspace_bytes(uint64_t m, uint64_t n, uint64_
 GF_EXPORT int gf_fp8_matmul(const gf_fp8_matmul_t* d, void* stream) {
     if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null descriptor");
     if (d->m == 0 || d->n == 0) return GF_OK;
-    if (!d->out) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null output");
-    if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: unknown dtype %u", d->dtype);
-    if (d->blocks == 0) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: no blocks to add up");
-    if (const char* e = operand_error(d->a, d->m)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: a: %s", e);
-    if (const char* e = operand_error(d->b, d->n)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: b: %s", e);
-    if (too_large(d->m, d->n, d->blocks)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: matrix too large (at most 65535 blocks along the sum)");
-    const Plan p = plan_of(d->m, d->n, d->blocks);
-    if (p.splits > 1 && (!d->workspace || (uintptr_t)d->workspace % 16)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_matmul: null or unaligned workspace");
-    MatmulArgs a;
-    a.a = {d->a.codes, d->a.scales, d->a.pitch, d->a.stride_row, d->a.stride_block};
-    a.b = {d->b.codes, d->b.scales, d->b.pitch, d->b.stride_row, d->b.stride_block};
-    a.m = (uint32_t)d->m; a.n = (uint32_t)d->n; a.blocks = (uint32_t)d->blocks;
-    a.per_split = p.per_split; a.tiles_m = p.tiles_m; a.tiles_n = p.tiles_n;
-    a.out = d->out;
-    const hipStream_t s = gf_stream(stream);
-    if (d->dtype == F32) launch_matmul<float>(a, p, d->workspace, s);
-    else if (d->dtype == BF16) launch_matmul<__bf16>(a, p, d->workspace, s);
-    else launch_matmul<_Float16>(a, p, d->workspace, s);
+    if (const int rc = matmul_error(*d)) return rc;
+    launch(*d, gf_stream(stream));
     return gf_check_launch("gf_fp8_matmul");
 }
 
@@ -464,8 +514,6 @@ GF_EXPORT int gf_fp8_rows(const gf_fp8_rows_t* d, void* stream) {
     const uint32_t groups = (uint32_t)((d->n + 15) / 16), wide = 1u << 20;      // a launch's work-items along x lie below 2^32
     const dim3 grid(groups < wide ? groups : wide, (groups + wide - 1) / wide);
     const hipStream_t s = gf_stream(stream);
-    if (d->dtype == F32) k_rows<float><<<grid, 64 * kRowWaves, 0, s>>>(*d);
-    else if (d->dtype == BF16) k_rows<__bf16><<<grid, 64 * kRowWaves, 0, s>>>(*d);
-    else k_rows<_Float16><<<grid, 64 * kRowWaves, 0, s>>>(*d);
+    with_type(d->dtype, [&](auto t) { k_rows<decltype(t)><<<grid, 64 * kRowWaves, 0, s>>>(*d); });
     return gf_check_launch("gf_fp8_rows");
 }

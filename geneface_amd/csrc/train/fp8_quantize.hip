@@ -6,18 +6,26 @@
 // 16 lanes: tiles are 32 rows then, without LDS, so that a few hundred rows still fill the chip.
 #include "../common.hpp"
 #include "fp8.hpp"
+#include "fp8_two.hpp"
 #include "geneface_train_hip.h"
 
 namespace gf {
 
 constexpr int kTile = 128;
 
+struct Scratch {
+    uint32_t most[4][kTile];                                           // a wave's largest magnitudes by column
+    uint8_t turned[kTile * kTile];
+};
+
+// tile `at` of a matrix
 template <typename T>
-__global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, const uint32_t blocks_r, const uint32_t blocks_c) {
-    __shared__ uint32_t most[4][kTile];                                // a wave's largest magnitudes by column
-    __shared__ __align__(16) uint8_t turned[kTile * kTile];
+__device__ __forceinline__ void quantize_tile(const gf_fp8_quantize_t& d, const uint32_t at, Scratch& lds) {
+    auto& most = lds.most;
+    uint8_t* turned = lds.turned;
+    const uint32_t blocks_r = (uint32_t)((d.rows + kTile - 1) / kTile), blocks_c = (uint32_t)((d.cols + kTile - 1) / kTile);
     const int t = threadIdx.x, j = t & 15, g = t >> 4, wave = t >> 6;  // columns 8j..8j+7 of the tile, rows 8g..8g+7
-    const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, br = at / blocks_c, bc = at % blocks_c;      // behind the last: rows that are not there
+    const uint32_t br = at / blocks_c, bc = at % blocks_c;
     if (br >= blocks_r) return;
     const uint64_t r0 = (uint64_t)br * kTile + 8 * g, c0 = (uint64_t)bc * kTile + 8 * j;
     const bool by_tile = d.tiles != 0;
@@ -95,6 +103,19 @@ __global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d, con
 }
 
 template <typename T>
+__global__ __launch_bounds__(256) void k_quantize(const gf_fp8_quantize_t d) {
+    __shared__ __align__(16) Scratch lds;
+    quantize_tile<T>(d, blockIdx.y * gridDim.x + blockIdx.x, lds);
+}
+
+template <typename A, typename B>
+__global__ __launch_bounds__(256) void k_quantize_two(const gf_fp8_quantize_t a, const gf_fp8_quantize_t b, const uint32_t tiles_a) {
+    __shared__ __align__(16) Scratch lds;
+    if (blockIdx.x < tiles_a) quantize_tile<A>(a, blockIdx.x, lds);
+    else quantize_tile<B>(b, blockIdx.x - tiles_a, lds);
+}
+
+template <typename T>
 __global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d, const uint32_t blocks_c) {
     const int j = threadIdx.x & 15, g = threadIdx.x >> 4;
     const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x, br = at / blocks_c, bc = at % blocks_c;      // behind the last: rows that are not there
@@ -115,11 +136,53 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const gf_fp8_quantize_t d
     }
 }
 
-template <typename T>
-static void launch_quantize(const gf_fp8_quantize_t& d, uint64_t rb, uint64_t cb, hipStream_t s) {
+static uint64_t tiles_of(const gf_fp8_quantize_t& d) { return ((d.rows + kTile - 1) / kTile) * ((d.cols + kTile - 1) / kTile); }
+static bool rows_alone(const gf_fp8_quantize_t& d) { return !d.col_codes && !d.tiles; }
+
+// f(T()) with the type that dtype names
+template <typename F>
+static void with_type(uint32_t dtype, F f) {
+    if (dtype == F32) f(float());
+    else if (dtype == BF16) f(__bf16());
+    else f(_Float16());
+}
+
+static void launch_quantize(const gf_fp8_quantize_t& d, hipStream_t s) {
     auto grid = [](uint64_t n) { const uint64_t wide = 1u << 22; return dim3((uint32_t)(n < wide ? n : wide), (uint32_t)((n + wide - 1) / wide)); };      // work-items along x lie below 2^32
-    if (!d.col_codes && !d.tiles) k_quantize_rows<T><<<grid((d.rows + 31) / 32 * cb), 256, 0, s>>>(d, (uint32_t)cb);
-    else k_quantize<T><<<grid(rb * cb), 256, 0, s>>>(d, (uint32_t)rb, (uint32_t)cb);
+    const uint64_t cb = (d.cols + kTile - 1) / kTile;
+    with_type(d.dtype, [&](auto t) {
+        if (rows_alone(d)) k_quantize_rows<decltype(t)><<<grid((d.rows + 31) / 32 * cb), 256, 0, s>>>(d, (uint32_t)cb);
+        else k_quantize<decltype(t)><<<grid(tiles_of(d)), 256, 0, s>>>(d);
+    });
+}
+
+static int quantize_error(const gf_fp8_quantize_t& d) {
+    if (!d.src || (!d.row_codes && !d.col_codes)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: null pointer");
+    if (d.tiles ? !d.tile_scales : ((d.row_codes && !d.row_scales) || (d.col_codes && !d.col_scales)))
+        return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: null scales");
+    if (d.dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: unknown dtype %u", d.dtype);
+    if (d.ld < d.cols) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: ld < cols");
+    if (!d.tiles && ((d.row_codes && d.row_pitch < d.rows) || (d.col_codes && d.col_pitch < d.cols)))
+        return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: scale pitch too small");
+    const uint64_t rb = (d.rows + kTile - 1) / kTile, cb = (d.cols + kTile - 1) / kTile;
+    if (rb > 0x1fffffffull || cb > 0x1fffffffull / rb) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: matrix too large");
+    return GF_OK;
+}
+
+int quantize_two(const gf_fp8_quantize_t& a, const gf_fp8_quantize_t& b, void* stream) {
+    if (const int rc = quantize_error(a)) return rc;
+    if (const int rc = quantize_error(b)) return rc;
+    const hipStream_t s = gf_stream(stream);
+    const uint64_t ta = tiles_of(a), tb = tiles_of(b);
+    if (rows_alone(a) || rows_alone(b) || ta + tb > 1u << 22) {
+        launch_quantize(a, s);
+        launch_quantize(b, s);
+    } else {
+        with_type(a.dtype, [&](auto x) {
+            with_type(b.dtype, [&](auto y) { k_quantize_two<decltype(x), decltype(y)><<<(uint32_t)(ta + tb), 256, 0, s>>>(a, b, (uint32_t)ta); });
+        });
+    }
+    return gf_check_launch("gf_fp8_quantize");
 }
 
 }  // namespace gf
@@ -129,18 +192,7 @@ using namespace gf;
 GF_EXPORT int gf_fp8_quantize(const gf_fp8_quantize_t* d, void* stream) {
     if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: null descriptor");
     if (d->rows == 0 || d->cols == 0) return GF_OK;
-    if (!d->src || (!d->row_codes && !d->col_codes)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: null pointer");
-    if (d->tiles ? !d->tile_scales : ((d->row_codes && !d->row_scales) || (d->col_codes && !d->col_scales)))
-        return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: null scales");
-    if (d->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: unknown dtype %u", d->dtype);
-    if (d->ld < d->cols) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: ld < cols");
-    if (!d->tiles && ((d->row_codes && d->row_pitch < d->rows) || (d->col_codes && d->col_pitch < d->cols)))
-        return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: scale pitch too small");
-    const uint64_t rb = (d->rows + kTile - 1) / kTile, cb = (d->cols + kTile - 1) / kTile;
-    if (rb > 0x1fffffffull || cb > 0x1fffffffull / rb) return gf_set_error(GF_ERR_INVALID, "gf_fp8_quantize: matrix too large");
-    const hipStream_t s = gf_stream(stream);
-    if (d->dtype == F32) launch_quantize<float>(*d, rb, cb, s);
-    else if (d->dtype == BF16) launch_quantize<__bf16>(*d, rb, cb, s);
-    else launch_quantize<_Float16>(*d, rb, cb, s);
+    if (const int rc = quantize_error(*d)) return rc;
+    launch_quantize(*d, gf_stream(stream));
     return gf_check_launch("gf_fp8_quantize");
 }

@@ -239,10 +239,7 @@ struct Linear : torch::autograd::Function<Linear> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, bool keep_w, bool keep_x) {
         Product p = ::forward(x, &w, nullptr, nullptr, w.size(0), keep_w, keep_x);
         ctx->save_for_backward({p.saved});
-        auto& s = ctx->saved_data;
-        s["m"] = x.size(0); s["k"] = x.size(1); s["n"] = w.size(0);
-        s["x_dtype"] = (int64_t)x.scalar_type(); s["w_dtype"] = (int64_t)w.scalar_type();
-        s["keep_w"] = keep_w; s["keep_x"] = keep_x; s["bytes"] = (int64_t)p.backward_bytes;
+        ctx->saved_data["plan"] = std::vector<int64_t>{x.size(0), x.size(1), w.size(0), (int64_t)x.scalar_type(), (int64_t)w.scalar_type(), keep_w, keep_x, (int64_t)p.backward_bytes};
         return p.y;
     }
 
@@ -250,17 +247,17 @@ struct Linear : torch::autograd::Function<Linear> {
         const bool again = at::GradMode::is_enabled();      // create_graph
         const at::AutoGradMode off(false);
         const Tensor saved = ctx->get_saved_variables()[0], dy = matrix(grads[0]);
-        auto& s = ctx->saved_data;
-        const int64_t m = s["m"].toInt(), k = s["k"].toInt(), n = s["n"].toInt();
+        const std::vector<int64_t> plan = ctx->saved_data["plan"].toIntVector();
+        const int64_t m = plan[0], k = plan[1], n = plan[2];
         const at::Device dev = dy.device();
         const c10::OptionalDeviceGuard guard(dev);
         Tensor dx, dw;
         gf_fp8_linear_backward_t d = {};
         d.dy = dy.data_ptr(); d.lddy = pitch(dy); d.saved = saved.data_ptr(); d.m = m; d.n = n; d.k = k;
-        d.keep_w = s["keep_w"].toBool(); d.keep_x = s["keep_x"].toBool();
-        if (d.keep_w && ctx->needs_input_grad(0)) dx = at::empty({m, k}, dy.options().dtype((at::ScalarType)s["x_dtype"].toInt()));
-        if (d.keep_x && ctx->needs_input_grad(1)) dw = at::empty({n, k}, dy.options().dtype((at::ScalarType)s["w_dtype"].toInt()));
-        const Tensor work = at::empty({s["bytes"].toInt()}, bytes_on(dev));
+        d.keep_w = plan[5]; d.keep_x = plan[6];
+        if (d.keep_w && ctx->needs_input_grad(0)) dx = at::empty({m, k}, dy.options().dtype((at::ScalarType)plan[3]));
+        if (d.keep_x && ctx->needs_input_grad(1)) dw = at::empty({n, k}, dy.options().dtype((at::ScalarType)plan[4]));
+        const Tensor work = at::empty({plan[7]}, bytes_on(dev));
         d.dx = dx.defined() ? dx.data_ptr() : nullptr;
         d.dw = dw.defined() ? dw.data_ptr() : nullptr;
         d.workspace = work.data_ptr();
