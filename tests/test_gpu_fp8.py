@@ -136,6 +136,32 @@ def test_types_of_their_own(tx, tw):
     _near(dw, gc.t() @ xc, gc.abs().t() @ xc.abs(), tw, 300, "dw")
 
 
+@pytest.mark.parametrize("tx", TYPES)
+@pytest.mark.parametrize("tw", TYPES)
+def test_every_pair_of_types(tx, tw):
+    """Sizes whose operands share a launch and whose gradients do; the weight's and x's magnitudes differ, so that a swap would show."""
+    x, w = _random(210, 140, tx, 1, 1.0).requires_grad_(True), (_random(170, 140, tw, 2, 1.0) / 64).requires_grad_(True)
+    y = fp8.linear(x, w)
+    dy = _random(210, 170, tx, 3, 1.0)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    xr, wt, gr, gc, xc = R.by_rows(x.detach()), R.by_tiles(w.detach()), R.by_rows(dy), R.by_columns(dy), R.by_columns(x.detach())
+    _near(y.detach(), xr @ wt.t(), xr.abs() @ wt.abs().t(), tx, 140, "y")
+    _near(dx, gr @ wt, gr.abs() @ wt.abs(), tx, 170, "dx")
+    _near(dw, gc.t() @ xc, gc.abs().t() @ xc.abs(), tw, 210, "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, N, K", [(200, 5000, 300), (1900, 2000, 257), (2500, 2450, 200), (4000, 4000, 129), (20, 90, 12000)])
+def test_every_tile(M, N, K, dtype):
+    """Results of so many tiles that each size of them is taken: 128 x 64, 128 x 128 with four blocks under way and with two, 256 x 256, and 64 x 64 with
+    a sum that is split.  Whole numbers: sums are exact, whatever their order."""
+    g = torch.Generator().manual_seed(M)
+    whole = lambda *s: torch.randint(-2, 3, s, generator=g).float().cuda()      # noqa: E731
+    x, w = whole(M, K), whole(N, K)
+    y = fp8.linear(x.to(dtype), fp8.quantize_weight(w))
+    assert torch.equal(y, (x.double() @ w.double().t()).to(dtype))
+
+
 def test_gradients_against_differences():
     """Along a direction the loss moves as the gradients say, on inputs that lie on the 8-bit grid with steps that stay on it: small whole numbers are
     exact in e4m3, so a difference of the quantised product is a difference of the product."""
