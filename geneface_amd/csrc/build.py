@@ -99,7 +99,7 @@ def _compile(src, force, extra=(), obj_dir=OBJ_DIR, drop=()):
 
 def build_host(force: bool = False) -> str:
     """_train_host.so: the operators' argument checks and calls in C++ against this interpreter's torch (lib.host() loads it)."""
-    newest = max(os.path.getmtime(p) for p in [HOST_SOURCE, __file__, train_headers()[-1]])
+    newest = max(os.path.getmtime(p) for p in [HOST_SOURCE, __file__, *train_headers()])
     if not force and os.path.exists(HOST_OUT) and os.path.getmtime(HOST_OUT) >= newest:
         return HOST_OUT
     import sysconfig

@@ -50,6 +50,7 @@ def _blocks(n):
 
 def _matrix(x):
     """x [..., K] as [M, K] whose rows are consecutive values, rows at any distance."""
+    x = x.resolve_neg()
     m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     return m if m.stride(1) == 1 and m.stride(0) >= m.shape[1] else m.contiguous()
 

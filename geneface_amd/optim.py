@@ -6,8 +6,8 @@ it.  With `weight_decay=0` it is Adam.
 
 8-bit moments: e4m3 codes with one 32-bit scale for each 128 consecutive values of a tensor, max(largest magnitude, 2^-100) times 1 / 448.  The second
 moment is held as its square root, which halves the range it needs.  Codes are rounded by a dither that depends on the step and on the value's
-index only, so a step is reproducible and changes far below the format's spacing add up over the steps; a second moment above zero never becomes
-zero.  A block that meets a gradient that is no finite number is none afterwards (all 128 values).
+index only, so a step is reproducible and changes far below the format's spacing add up over the steps; a second moment above zero is never rounded
+to zero.  A block that meets a gradient that is no finite number is none afterwards (all 128 values).
 
 Everything is done on the current stream of the tensors' device and may be captured into a graph; a graph keeps the addresses, and numbers given
 as Python numbers (`lr` as a one-element tensor on the device stays adjustable).
@@ -54,7 +54,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
 
     params, grads: float32, bfloat16 or float16, gradients of their parameter's type and size.  exp_avgs, exp_avg_sqs: float32 of the same sizes,
     or -- with exp_avg_scales and exp_avg_sq_scales, lists of float32 [ceil(numel / 128)] -- float8_e4m3fn.  steps: one float32 each, the number of
-    steps taken so far.  Everything on one device; all but gradients must be contiguous.
+    steps taken so far.  Everything on one device; all but gradients must be contiguous, and no two of them may share memory.
 
     lr: a number, or one float32 on the device.  grad_scale: the factor that the gradients carry.  found_inf: where it is not 0 nothing is
     changed, the step counts included.  grad_norm, max_norm: gradients are multiplied by min(1, max_norm / (grad_norm + 1e-6)); both or neither.
@@ -79,7 +79,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32, or 8 for moments of one byte each and a scale per 128 values (16 bytes moved per float32 parameter instead of 28).
     max_grad_norm: clips the gradients of ALL groups to this norm inside the step; the norm of the last step stays in `last_grad_norm`.  The
     gradients themselves are not changed.  Under torch.amp.GradScaler unscaling and the skipped step after an overflow happen inside the kernel, without a
-    host sync.  lr may be a one-element float32 tensor on the device, so that a captured step follows a schedule."""
+    host sync.  lr may be a one-element float32 tensor on the device, so that a captured step follows a schedule; a parameter's first step is not captured."""
 
     _step_supports_amp_scaling = True      # GradScaler.step hands its scale and found_inf over as attributes and calls step() itself
 
@@ -110,6 +110,8 @@ class AdamW(torch.optim.Optimizer):
         if not state:
             if p.dtype not in DTYPES or not p.is_cuda or not p.is_contiguous():
                 raise RuntimeError("AdamW: parameters must be contiguous CUDA tensors of float32, bfloat16 or float16")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a parameter's first step cannot be captured (every replay would start its state anew): take one before, or load a state")
             state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
             for k in self._keys():
                 if k.endswith("scale"):
@@ -167,17 +169,20 @@ class AdamW(torch.optim.Optimizer):
             missing = [k for k in ("step", *want) if k not in s]
             if missing or any(s[k].dtype != dt for k, dt in want.items()):
                 raise RuntimeError(f"AdamW: the state does not hold {self.state_bits}-bit moments")
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize") or (g.get("weight_decay") and not g.get("decoupled_weight_decay", True)):
+                raise RuntimeError("AdamW: a state with amsgrad, maximize or Adam's own weight decay belongs to another update")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        super().load_state_dict(state_dict)
         params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            for k in want if i in state_dict["state"] else ():
+                held, shape = tuple(state_dict["state"][i][k].shape), (-(-p.numel() // BLOCK),) if k.endswith("scale") else tuple(p.shape)
+                if held != shape:
+                    raise RuntimeError(f"AdamW: {k} of shape {held} for a parameter of shape {tuple(p.shape)}")
+        super().load_state_dict(state_dict)
         for i, p in zip(ids, params):
             s = state_dict["state"].get(i)
             if s is None:
                 continue
-            state = {"step": torch.as_tensor(s["step"], dtype=torch.float32).detach().to(p.device, copy=True).reshape(())}
-            for k in want:
-                shape = (-(-p.numel() // BLOCK),) if k.endswith("scale") else p.shape
-                if tuple(s[k].shape) != tuple(shape):
-                    raise RuntimeError(f"AdamW: {k} of shape {tuple(s[k].shape)} for a parameter of shape {tuple(p.shape)}")
-                state[k] = s[k].detach().to(p.device, copy=True).contiguous()
-            self.state[p] = state
+            self.state[p] = {"step": torch.as_tensor(s["step"], dtype=torch.float32).detach().to(p.device, copy=True).reshape(()),
+                             **{k: s[k].detach().to(p.device, copy=True).contiguous() for k in want}}

@@ -212,6 +212,17 @@ def test_shapes_strides_and_emptiness():
     assert torch.equal(*ga)
 
 
+def test_values_whose_sign_is_still_to_be_applied():
+    c = torch.complex(_random(40, 200, torch.float32, 1), _random(40, 200, torch.float32, 2)).conj()
+    x, w = c.imag, _random(30, 200, torch.float32, 3)
+    assert x.is_neg()
+    y = fp8.linear(x, w)
+    assert torch.equal(y, fp8.linear(-c.conj().imag.contiguous(), w)) and bool(y.any())
+    assert torch.equal(fp8.linear(x, fp8.quantize_weight(w)), y)
+    v = c[:30].imag
+    assert torch.equal(fp8.linear(w, v), fp8.linear(w, v.clone())) and torch.equal(fp8.linear(w, fp8.quantize_weight(v)), fp8.linear(w, v))
+
+
 def test_gradient_that_is_expanded():
     x, w = _random(200, 150, torch.float32, 1).requires_grad_(True), _random(100, 150, torch.float32, 2).requires_grad_(True)
     y = fp8.linear(x, w)

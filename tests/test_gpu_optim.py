@@ -389,6 +389,66 @@ def test_the_same_tensor_twice_is_refused():
     assert all(float(x.abs().max()) == 0 for x in a)
 
 
+def test_tensors_that_share_memory_are_refused():
+    flat = torch.zeros(40, device="cuda")
+    z = lambda n: [torch.zeros(n, device="cuda") for _ in range(2)]      # noqa: E731
+    steps = [torch.zeros((), device="cuda") for _ in range(2)]
+    with pytest.raises(RuntimeError, match="share memory"):
+        optim.adamw_step([flat[:10], flat[9:19]], z(10), z(10), z(10), steps, lr=1.0)
+    with pytest.raises(RuntimeError, match="share memory"):
+        optim.adamw_step([flat[:10], flat[20:30]], z(10), [flat[29:39], z(10)[0]], z(10), steps, lr=1.0)
+    many, n = torch.zeros(200, 8, device="cuda"), 40
+    rows = lambda: list(torch.zeros(n, 8, device="cuda"))      # noqa: E731
+    for at in range(0, n, 13):      # one of many, at some place among the others
+        p = [many[5 * i] for i in range(n)]
+        p[at] = many[5 * ((at + 7) % n)].view(-1)[:3] if at else many.view(-1)[5 * 8 * 7 + 4:5 * 8 * 7 + 12]
+        like = lambda: [torch.zeros_like(x) for x in p]      # noqa: E731
+        with pytest.raises(RuntimeError, match="share memory"):
+            optim.adamw_step(p, like(), like(), like(), list(torch.zeros(n, device="cuda")), lr=1.0)
+    optim.adamw_step([many[5 * i] for i in range(n)], rows(), rows(), rows(), list(torch.zeros(n, device="cuda")), lr=1.0)
+    optim.adamw_step([flat[:10], flat[10:20]], [torch.ones(10, device="cuda")] * 2, z(10), z(10), steps, lr=1.0, weight_decay=0.0)
+    assert bool((flat[:20] < -0.9).all()) and not bool(flat[20:].any())
+
+
+def test_a_gradient_whose_sign_is_still_to_be_applied():
+    c = torch.randn(300, dtype=torch.complex64, generator=_gen(3)).cuda()
+    g = c.conj().imag
+    assert g.is_neg()
+    got = []
+    for grad in (g, g.clone().contiguous() + 0.0):
+        p, m, v = (torch.zeros(300, device="cuda") for _ in range(3))
+        optim.adamw_step([p], [grad], [m], [v], [torch.zeros((), device="cuda")], lr=0.1)
+        got.append(p)
+    assert torch.equal(*got) and bool((got[0] != 0).any())
+
+
+def test_a_first_step_is_not_captured(monkeypatch):
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    p.grad = torch.ones(5, device="cuda")
+    o = optim.AdamW([p])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="first step"):
+        o.step()
+    monkeypatch.undo()
+    o.step()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    o.step()
+    assert float(o.state[p]["step"]) == 2
+
+
+@pytest.mark.parametrize("g", [1e-15, 1e-21, 1e-25])
+def test_gradients_far_below_the_range_of_their_squares(g):
+    """g^2 is a subnormal number, or nothing: the second moment is the root of what a 32-bit square leaves of it, between nothing and its value."""
+    p, grad = torch.zeros(256, device="cuda"), torch.full((256,), g, device="cuda")
+    m, v = (torch.zeros(256, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+    ms, vs = (torch.zeros(2, device="cuda") for _ in range(2))
+    optim.adamw_step([p], [grad], [m], [v], [torch.zeros((), device="cuda")], lr=0.1, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    first, root = m.float() * ms[0], v.float() * vs[0]
+    assert bool(((first / (0.1 * g) - 1).abs() <= 2.0 ** -3).all())                      # a code is at most a spacing below or above
+    assert bool((root <= 0.1 * g * (1 + 2.0 ** -3) + 448 * 2.0 ** -100 / 448).all()) and bool((root >= 0).all())
+    assert float(p.abs().max()) <= 0.1 * g / 1e-8 * 1.01
+
+
 def _written_out(q, scale, n):
     return q.float().cpu() * scale.cpu().repeat_interleave(128)[:n]
 

@@ -108,6 +108,30 @@ def test_state_of_torch_adam_loads_and_keeps_its_types():
         o.load_state_dict({"state": {0: {"step": 7, "exp_avg": m[:2], "exp_avg_sq": v}}, "param_groups": o.state_dict()["param_groups"]})
 
 
+@pytest.mark.parametrize("group", [dict(amsgrad=True), dict(maximize=True), dict(weight_decay=0.1, decoupled_weight_decay=False)])
+def test_state_of_another_update_is_refused(group):
+    p = torch.nn.Parameter(torch.zeros(3))
+    o = optim.AdamW([p], lr=0.5)
+    d = o.state_dict()
+    d["param_groups"][0].update(group, lr=0.25)
+    with pytest.raises(RuntimeError, match="another update"):
+        o.load_state_dict(d)
+    assert o.param_groups[0]["lr"] == 0.5
+    d["param_groups"][0].update(dict.fromkeys(group, False), weight_decay=0.0)
+    o.load_state_dict(d)
+    assert o.param_groups[0]["lr"] == 0.25
+
+
+def test_a_refused_state_leaves_the_old_one():
+    p = torch.nn.Parameter(torch.zeros(3, 2))
+    o = optim.AdamW([p])
+    held = {"step": 3, "exp_avg": torch.ones(3, 2), "exp_avg_sq": torch.ones(3, 2)}
+    o.load_state_dict({"state": {0: held}, "param_groups": o.state_dict()["param_groups"]})
+    with pytest.raises(RuntimeError, match="of shape"):
+        o.load_state_dict({"state": {0: {**held, "step": 9, "exp_avg_sq": torch.ones(2, 3)}}, "param_groups": o.state_dict()["param_groups"]})
+    assert float(o.state[p]["step"]) == 3
+
+
 def test_the_library_refuses_bad_descriptors(hip_lib):
     def refused(rc, word):
         assert rc == 1 and word in hip_lib.gf_last_error(), hip_lib.gf_last_error()
