@@ -5,7 +5,8 @@
 namespace gf {
 
 // out = the sum of the splits' parts in a fixed order: a wave adds up every WAVES-th of them for 256 values, then the waves' sums are added.  Eight
-// loads are under way at a time: the parts of a tall product's weight gradient are hundreds, of few values each, and latency is all they cost.
+// loads are under way at a time: the parts of a tall product's weight gradient are hundreds, of few values each, and latency is all they cost
+// (512 parts of 128 x 96: 8 us).
 template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_join(const float* part, uint32_t splits, uint64_t count, T* out) {
     __shared__ f32x4 sums[WAVES][64];

