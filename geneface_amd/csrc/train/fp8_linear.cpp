@@ -1,12 +1,12 @@
 // gf_fp8_linear and gf_fp8_linear_backward: a layer's products with what they need around them, as one call each.  Host code over the entry points of
 // fp8_quantize.hip and fp8_matmul.hip; what it decides is where everything lies in the caller's two buffers.
 #include "../common.hpp"
-#include "fp8_two.hpp"
+#include "fp8_calls.hpp"
 #include "geneface_train_hip.h"
 
 namespace gf {
 
-// One block of 128 on either side: gf_fp8_thin (262221 rows, 96 -> 128, 32 bits, both directions: 129 us, by the general path 179).
+// One block of 128 on either side: gf_fp8_thin (262221 rows, 96 -> 128, 32 bits, both directions: 126 us, by the general path 179).
 static bool thin(uint64_t n, uint64_t k) { return n <= 128 && k <= 128; }
 
 static uint64_t blocks_of(uint64_t n) { return (n + 127) / 128; }
@@ -36,11 +36,10 @@ struct Forward { uint8_t *x_codes, *x_scales, *w_codes, *w_scales, *parts; };
 static Forward forward_pieces(Pieces& p, const gf_fp8_linear_t& d) {
     Forward f = {};
     if (!d.w && d.m <= 16) return f;      // gf_fp8_rows needs nothing
-    if (!thin(d.n, d.k)) {
-        f.x_codes = p.take(d.m * blocks_of(d.k) * 128);
-        f.x_scales = p.take(blocks_of(d.k) * d.m);
-        f.parts = p.take(gf_fp8_matmul_workspace_bytes(d.m, d.n, blocks_of(d.k)));
-    }
+    if (thin(d.n, d.k)) return f;         // and neither does gf_fp8_thin
+    f.x_codes = p.take(d.m * blocks_of(d.k) * 128);
+    f.x_scales = p.take(blocks_of(d.k) * d.m);
+    f.parts = p.take(gf_fp8_matmul_workspace_bytes(d.m, d.n, blocks_of(d.k)));
     if (d.w) f.w_codes = p.take(d.n * blocks_of(d.k) * 128);
     if (d.w && !d.keep_w) f.w_scales = p.take(blocks_of(d.n) * blocks_of(d.k));
     return f;
@@ -113,7 +112,7 @@ GF_EXPORT int gf_fp8_linear(const gf_fp8_linear_t* d, void* stream) {
         const gf_fp8_rows_t r = {d->x, d->m, d->n, d->k, d->ldx, d->codes, d->scales, d->y, d->dtype, 0};
         return gf_fp8_rows(&r, stream);
     }
-    if ((!d->workspace && (d->w || !thin(d->n, d->k))) || ((d->keep_w || d->keep_x) && !d->saved)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: null buffer");
+    if ((!d->workspace && !thin(d->n, d->k)) || ((d->keep_w || d->keep_x) && !d->saved)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: null buffer");
     if ((uintptr_t)d->workspace % 256 || (uintptr_t)d->saved % 256) return gf_set_error(GF_ERR_INVALID, "gf_fp8_linear: buffers must start at multiples of 256 bytes");
     Pieces ps{(uint8_t*)d->saved}, pf{(uint8_t*)d->workspace};
     const Saved s = saved_pieces(ps, d->m, d->n, d->k, d->keep_w, d->keep_x);
@@ -123,10 +122,9 @@ GF_EXPORT int gf_fp8_linear(const gf_fp8_linear_t* d, void* stream) {
     const gf_fp8_quantize_t qw = {d->w, d->n, d->k, d->ldw, d->w_dtype, 1, f.w_codes, nullptr, s.w_codes, nullptr, d->keep_w ? s.w_scales : f.w_scales, 0, 0};
     const gf_fp8_quantize_t qx = {d->x, d->m, d->k, d->ldx, d->dtype, 0, f.x_codes, f.x_scales, s.x_codes, s.x_scales, nullptr, d->m, d->k};
     if (thin(d->n, d->k)) {
-        if (d->w)
-            if (const int rc = gf_fp8_quantize(&qw, stream)) return rc;
         const gf_fp8_thin_t t = {d->x, d->ldx, d->m, d->n, d->k, w_codes, w_scales, d->y, s.x_codes, s.x_scales, d->dtype, 0};
-        return gf_fp8_thin(&t, stream);
+        const ThinWeight w = {d->w, d->ldw, d->w_dtype, s.w_codes, s.w_scales};
+        return thin_forward(t, d->w ? &w : nullptr, stream);
     }
     if (const int rc = d->w ? quantize_two(qw, qx, stream) : gf_fp8_quantize(&qx, stream)) return rc;
     const gf_fp8_matmul_t p = {{f.x_codes, f.x_scales, d->m, 0, 0}, {w_codes, w_scales, 0, kb, 1}, d->m, d->n, kb, d->y, d->dtype, 0, f.parts};

@@ -5,8 +5,8 @@
 // they reach a lane does not matter as long as both operands have the same.
 #include "../common.hpp"
 #include "fp8.hpp"
+#include "fp8_calls.hpp"
 #include "fp8_join.hpp"
-#include "fp8_two.hpp"
 #include "geneface_train_hip.h"
 #include <type_traits>
 #include <utility>

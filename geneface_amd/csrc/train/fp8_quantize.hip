@@ -7,7 +7,7 @@
 // 18 us (5.5 TB/s); 4096 x 4096 both ways, float32 as a weight and bfloat16 as its input in one launch, in 31-36 us (168 MB, 4.7-5.4 TB/s).
 #include "../common.hpp"
 #include "fp8.hpp"
-#include "fp8_two.hpp"
+#include "fp8_calls.hpp"
 #include "geneface_train_hip.h"
 
 namespace gf {

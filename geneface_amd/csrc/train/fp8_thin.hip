@@ -6,9 +6,10 @@
 // avoid: a workgroup brings its 128 rows to 8 bits in LDS and multiplies them there.  The weight's codes stay in LDS for all its tiles.  Forward: x is
 // read once, y and (for the weight's gradient) x by columns are written.  Backward: dy is read once for both products; the weight's gradient is
 // added up in the registers of the workgroup over all its tiles, so that only a part per workgroup has to be joined.
-// Measured, 262221 rows, 96 -> 128, float32: forward 54-57 us (268 MB, 4.8 TB/s), backward 61-64 (293 MB, 4.7 TB/s), the join of its 512 parts 8.
+// Measured, 262221 rows, 96 -> 128, float32: forward 57-62 us with the weight's own quantisation (268 MB, 4.3-4.7 TB/s), backward 61-64 (293 MB, 4.7 TB/s), the join of its 512 parts 8.
 #include "../common.hpp"
 #include "fp8.hpp"
+#include "fp8_calls.hpp"
 #include "fp8_join.hpp"
 #include "geneface_train_hip.h"
 
@@ -167,19 +168,56 @@ struct ThinForward {
     const uint8_t *w_codes, *w_scale;      // [n, 128] and one byte
     void* y;
     uint8_t *col_codes, *col_scales;       // x by columns [k, 128 tiles] and [tiles, k], or NULL
+    ThinWeight w;                          // the weight as values, or w.w NULL
 };
 
+// The weight's values to its codes in LDS, by every workgroup for itself (48 KB out of L2; a launch ahead that does it once
+// takes 6 us), and by the first one for the backward call.  Returns the scale's byte.
+template <typename W>
+__device__ __forceinline__ uint32_t weight_to(uint8_t* weight, uint8_t* turned, uint32_t most[4][kEdge], uint8_t* scales, const ThinForward& d) {
+    Tile<W> w;
+    w.load((const W*)d.w.w, d.w.ldw, 0, d.n, d.k);
+    uint32_t m = 0;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) m = max(m, w.x[r].amax());
+    m = row_max_u32(m);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6][0] = m;
+    __syncthreads();
+    const uint32_t byte = scale_byte(max(max(most[0][0], most[1][0]), max(most[2][0], most[3][0])));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.rows[i] = w.cols[i] = byte;
+    w.row_codes_to(weight, scales);
+    if (blockIdx.x == 0 && d.w.col_codes) {
+        w.column_codes_to(turned);
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int c = q * 32 + (threadIdx.x >> 3), p = threadIdx.x & 7;
+            if (c < (int)d.k) *reinterpret_cast<i32x4*>(d.w.col_codes + c * kEdge + p * 16) = *reinterpret_cast<const i32x4*>(turned + spot(c, p));
+        }
+        if (threadIdx.x == 0) *d.w.scale = (uint8_t)byte;
+    }
+    return byte;
+}
+
+// (Three workgroups a CU, as its LDS holds, cost the 32-bit form eight registers of scratch: 126 us for the layer, with two workgroups 129.)
 template <typename T>
-__global__ __launch_bounds__(256) void k_thin_forward(const ThinForward d) {
+__global__ __launch_bounds__(256, 3) void k_thin_forward(const ThinForward d) {
     __shared__ __align__(16) uint8_t weight[kEdge * kEdge], codes[kEdge * kEdge], turned[kEdge * kEdge];
     __shared__ uint32_t most[4][kEdge];
     __shared__ uint8_t scales[kEdge];
-    {
+    uint32_t sw;
+    if (d.w.w) {
+        sw = d.w.dtype == F32 ? weight_to<float>(weight, turned, most, scales, d) : d.w.dtype == BF16 ? weight_to<__bf16>(weight, turned, most, scales, d)
+                                                                                                      : weight_to<_Float16>(weight, turned, most, scales, d);
+    } else {
         CodesTile w;
         w.load(d.w_codes, kEdge, d.n);
         w.to(weight);
+        sw = *d.w_scale;
     }
-    const uint32_t sw = *d.w_scale;
     __syncthreads();
     for (uint32_t t = blockIdx.x; t < d.tiles; t += gridDim.x) {
         const uint64_t r0 = (uint64_t)t * kEdge;
@@ -315,23 +353,29 @@ static int thin_error(const char* what, uint64_t m, uint64_t n, uint64_t k, uint
     return GF_OK;
 }
 
+int thin_forward(const gf_fp8_thin_t& d, const ThinWeight* w, void* stream) {
+    if (const int rc = thin_error("gf_fp8_thin", d.m, d.n, d.k, d.dtype)) return rc;
+    if (!d.x || (w ? !w->w || (!w->col_codes) != (!w->scale) : !d.codes || !d.scale) || !d.y || (!d.col_codes) != (!d.col_scales))
+        return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: null pointer");
+    if ((uintptr_t)(w ? w->col_codes : d.codes) % 16 || (uintptr_t)d.col_codes % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: codes must start at a multiple of 16 bytes");
+    if (d.ldx < d.k || (w && w->ldw < d.k)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: ldx < k");
+    if (w && w->dtype > F16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: unknown dtype %u", w->dtype);
+    const uint32_t tiles = (uint32_t)((d.m + kEdge - 1) / kEdge), grid = groups_of(tiles, 3);
+    const ThinForward a = {d.x, d.ldx, d.m, (uint32_t)d.n, (uint32_t)d.k, tiles, d.codes, d.scale, d.y, d.col_codes, d.col_scales, w ? *w : ThinWeight{}};
+    const hipStream_t s = gf_stream(stream);
+    if (d.dtype == F32) k_thin_forward<float><<<grid, 256, 0, s>>>(a);
+    else if (d.dtype == BF16) k_thin_forward<__bf16><<<grid, 256, 0, s>>>(a);
+    else k_thin_forward<_Float16><<<grid, 256, 0, s>>>(a);
+    return gf_check_launch("gf_fp8_thin");
+}
+
 }  // namespace gf
 
 using namespace gf;
 
 GF_EXPORT int gf_fp8_thin(const gf_fp8_thin_t* d, void* stream) {
     if (!d) return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: null descriptor");
-    if (const int rc = thin_error("gf_fp8_thin", d->m, d->n, d->k, d->dtype)) return rc;
-    if (!d->x || !d->codes || !d->scale || !d->y || (!d->col_codes) != (!d->col_scales)) return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: null pointer");
-    if ((uintptr_t)d->codes % 16 || (uintptr_t)d->col_codes % 16) return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: codes must start at a multiple of 16 bytes");
-    if (d->ldx < d->k) return gf_set_error(GF_ERR_INVALID, "gf_fp8_thin: ldx < k");
-    const uint32_t tiles = (uint32_t)((d->m + kEdge - 1) / kEdge), grid = groups_of(tiles, 3);
-    const ThinForward a = {d->x, d->ldx, d->m, (uint32_t)d->n, (uint32_t)d->k, tiles, d->codes, d->scale, d->y, d->col_codes, d->col_scales};
-    const hipStream_t s = gf_stream(stream);
-    if (d->dtype == F32) k_thin_forward<float><<<grid, 256, 0, s>>>(a);
-    else if (d->dtype == BF16) k_thin_forward<__bf16><<<grid, 256, 0, s>>>(a);
-    else k_thin_forward<_Float16><<<grid, 256, 0, s>>>(a);
-    return gf_check_launch("gf_fp8_thin");
+    return thin_forward(*d, nullptr, stream);
 }
 
 GF_EXPORT uint64_t gf_fp8_thin_workspace_bytes(uint64_t m, uint64_t n, uint64_t k) {
