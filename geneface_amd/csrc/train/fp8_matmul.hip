@@ -54,8 +54,9 @@ constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 
 // read as zero).  Row r is 128 bytes, its 16-byte piece c at place c ^ ((r >> 1) & 7), so that the same piece of any 16 consecutive rows lies on
 // different banks.  A step multiplies one block in two halves of 64, and the fragments of a half are read from LDS while the half before it is
 // multiplied, so the matrix unit waits for nothing but the one barrier of a step: behind it everyone has read the block, whose place the block
-// STAGES further on is then loaded into.  With one wave on each SIMD there is nobody else to fill a gap, hence the interleaving by hand (weave): one
-// LDS read and one load beside each matrix instruction.
+// STAGES further on is then loaded into.  With one wave on each SIMD there is nobody else to fill a gap, hence the interleaving by hand (weave): an
+// LDS read or two and a load beside each matrix instruction.  (Two waves on each, with 128 x 64 each of a tile of 256, take as long: 104 us for 4096 x 4096 x
+// 8192, 233 against 223 for 8192 x 8192 x 4096.)
 //
 // Measured: m 8192, n 8192, k 4096 to bfloat16 in 222-250 us (2 200-2 480 TFLOP/s; the library's tensor-scaled product 226), 4096 each 58-65; to float32 (EXACT)
 // 4096 each 106-116 us (1 180-1 300 TFLOP/s).  The matrix units are busy for two thirds of a wave's life; the rest is the barrier of a step, first loads and last stores.
@@ -182,7 +183,8 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& d, const uint32_t 
     };
     auto weave = [&](auto loads) __attribute__((always_inline)) {
         constexpr int MF = TM * TN * (EXACT ? 4 : 1), DS = 2 * (TM + TN), LD = LA + LB;
-        constexpr int per_ds = DS > MF ? DS / MF : 1, per_ld = LD > MF ? LD / MF : 1;
+        // the reads beside the first half of the matrix instructions, so that the last of them is back when those are through (512 x 4096 x 4096: 13.8 -> 13.4 us)
+        constexpr int per_ds = 2 * DS > MF ? 2 * DS / MF : 1, per_ld = LD > MF ? LD / MF : 1;
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                          // a matrix instruction,
