@@ -298,6 +298,45 @@ def test_captured_and_replayed():
             assert all(torch.equal(a, b.detach()) for a, b in zip(out, run(*c))), i
 
 
+@pytest.mark.parametrize("M, N, K", [(300, 140, 150), (30, 90, 12000), (2000, 200, 4000)])
+def test_two_captured_graphs_of_one_pool(M, N, K):
+    """Operands and gradients that share launches, sums that are split (their parts in a workspace of the call): two graphs out of one pool, replayed in
+    turn with eager work between, give what the eager calls give."""
+    w = _random(N, K, torch.float32, 2, 1.0) / math.sqrt(K)
+    q = fp8.quantize_weight(w)
+
+    def make(seed):
+        return _random(M, K, torch.bfloat16, seed, 1.0).requires_grad_(True), w.clone().requires_grad_(True), _random(M, N, torch.bfloat16, seed + 1, 1.0)
+
+    def run(x, v, dy):
+        y = fp8.linear(x, v)
+        return [y.detach(), *torch.autograd.grad(y, (x, v), dy), fp8.linear(x.detach(), q)]
+    cases, graphs, outs, pool = [make(10), make(20)], [], [], None
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in cases:
+            run(*c)
+    torch.cuda.current_stream().wait_stream(side)
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(run(*c))
+        pool = graph.pool()
+        graphs.append(graph)
+    for i in range(3):
+        with torch.no_grad():
+            for c in cases:
+                c[0].mul_(0.9)
+                c[1].mul_(1.1)
+                c[2].add_(0.01)
+        want = [run(*c) for c in cases]
+        for graph, out, right in zip(graphs, outs, want):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, right)), i
+
+
 def test_on_two_streams():
     q = fp8.quantize_weight(_random(1000, 3000, torch.float32, 2))
     xs = [_random(m, 3000, torch.bfloat16, m) for m in (200, 9, 300, 16)]
