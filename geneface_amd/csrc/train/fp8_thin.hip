@@ -6,7 +6,7 @@
 // avoid: a workgroup brings its 128 rows to 8 bits in LDS and multiplies them there.  The weight's codes stay in LDS for all its tiles.  Forward: x is
 // read once, y and (for the weight's gradient) x by columns are written.  Backward: dy is read once for both products; the weight's gradient is
 // added up in the registers of the workgroup over all its tiles, so that only a part per workgroup has to be joined.
-// Measured, 262221 rows, 96 -> 128, float32: forward 57-62 us with the weight's own quantisation (268 MB, 4.3-4.7 TB/s), backward 61-64 (293 MB, 4.7 TB/s), the join of its 512 parts 8.
+// Measured, 262221 rows, 96 -> 128, float32: forward 51-56 us with the weight's own quantisation (268 MB, 4.8-5.3 TB/s), backward 60-66 (293 MB, 4.4-4.9 TB/s), the join of its 512 parts 8.
 #include "../common.hpp"
 #include "fp8.hpp"
 #include "fp8_calls.hpp"
@@ -90,7 +90,9 @@ struct Tile {
         }
     }
     __device__ __forceinline__ void column_codes_to(uint8_t* tile) const {
-        const int c0 = 8 * (threadIdx.x & 15), g = threadIdx.x >> 4;
+        int t = threadIdx.x;
+        asm volatile("" : "+v"(t));      // its places are worked out here, not kept in registers over all tiles: three workgroups' have to fit a CU
+        const int c0 = 8 * (t & 15), g = t >> 4;
 #pragma unroll
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint2*>(tile + spot(c0 + c, g >> 1) + (g & 1) * 8) = coded(encode_column(x, c, scale_value(cols[c])), cols[c]);
     }
@@ -202,7 +204,7 @@ __device__ __forceinline__ uint32_t weight_to(uint8_t* weight, uint8_t* turned, 
     return byte;
 }
 
-// (Three workgroups a CU, as its LDS holds, cost the 32-bit form eight registers of scratch: 126 us for the layer, with two workgroups 129.)
+// Three workgroups a CU, as its LDS holds: 120 us for the layer in 32 bits, with two 129.
 template <typename T>
 __global__ __launch_bounds__(256, 3) void k_thin_forward(const ThinForward d) {
     __shared__ __align__(16) uint8_t weight[kEdge * kEdge], codes[kEdge * kEdge], turned[kEdge * kEdge];
@@ -224,6 +226,7 @@ __global__ __launch_bounds__(256, 3) void k_thin_forward(const ThinForward d) {
         Tile<T> x;
         x.load((const T*)d.x, d.ldx, r0, d.m, d.k);
         x.scale_rows();
+        x.row_codes_to(codes, scales);      // a wave's own rows: no barrier between writing and reading them
         if (d.col_codes) {
             x.columns_to(most);
             __syncthreads();      // also: everyone is done with the last tile
@@ -237,7 +240,6 @@ __global__ __launch_bounds__(256, 3) void k_thin_forward(const ThinForward d) {
                 }
             }
         }
-        x.row_codes_to(codes, scales);      // a wave's own rows: no barrier between writing and reading them
         __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_wave_barrier();
         if (d.col_codes) {
