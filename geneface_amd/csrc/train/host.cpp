@@ -10,10 +10,12 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
 #include <cstring>
+#include <deque>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -24,8 +26,33 @@
 
 namespace {
 
+namespace py = pybind11;
 using at::Tensor;
-using Tensors = std::vector<Tensor>;
+
+// The tensors of a Python list or tuple where they lie in their Python objects, which the sequence holds as long as the call takes.  A vector of tensors
+// would count every one's references up and down again: 24 tensors of 32 bits take 8.0 us so, 10.3 that way; 200 take 36 for 57.
+struct Tensors {
+    py::object sequence;
+    std::vector<const Tensor*> at;
+    std::deque<Tensor> own;      // those that replace one of the caller's
+
+    explicit Tensors(const py::object& given) : sequence(py::reinterpret_steal<py::object>(PySequence_Fast(given.ptr(), "a list of tensors is needed"))) {
+        if (!sequence) throw py::error_already_set();
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(sequence.ptr());
+        PyObject** items = PySequence_Fast_ITEMS(sequence.ptr());
+        at.reserve(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            if (!THPVariable_Check(items[i])) throw py::type_error("a list of tensors is needed");
+            at.push_back(&THPVariable_Unpack(items[i]));
+        }
+    }
+    size_t size() const { return at.size(); }
+    const Tensor& operator[](size_t i) const { return *at[i]; }
+    void replace(size_t i, Tensor t) {
+        own.push_back(std::move(t));
+        at[i] = &own.back();
+    }
+};
 
 struct Api {
     int (*adamw_step)(const gf_adamw_t*, void*);
@@ -73,13 +100,13 @@ void* stream_of(const at::Device& d) { return c10::hip::getCurrentHIPStream(d.in
 
 void same_device(const char* what, const Tensors& list, const at::Device& d) {
     if (d.type() != at::kCUDA) throw std::runtime_error(std::string(what) + " must be CUDA tensors");
-    for (const Tensor& t : list)
-        if (t.device() != d) throw std::runtime_error(std::string(what) + " must all be on " + name_of(d));
+    for (const Tensor* t : list.at)
+        if (t->device() != d) throw std::runtime_error(std::string(what) + " must all be on " + name_of(d));
 }
 
 void strided(const char* what, const Tensors& list) {
-    for (const Tensor& t : list)
-        if (t.layout() != at::kStrided) throw std::runtime_error(std::string(what) + ": sparse gradients are not supported");
+    for (const Tensor* t : list.at)
+        if (t->layout() != at::kStrided) throw std::runtime_error(std::string(what) + ": sparse gradients are not supported");
 }
 
 // t as its memory has to be: consecutive values, no sign left to be applied (a view such as conj().imag carries one)
@@ -120,10 +147,14 @@ void sort_by_address(std::vector<Span>& spans) {
 
 // ---- AdamW ---------------------------------------------------------------------------------------------------------------------------------
 
-void adamw_step(const Tensors& params, Tensors grads, const Tensors& m, const Tensors& v, const Tensors& steps, double lr, const std::optional<Tensor>& lr_device,
-                double beta1, double beta2, double eps, double weight_decay, const std::optional<Tensors>& m_scales, const std::optional<Tensors>& v_scales,
+void adamw_step(const py::object& params_, const py::object& grads_, const py::object& m_, const py::object& v_, const py::object& steps_, double lr,
+                const std::optional<Tensor>& lr_device, double beta1, double beta2, double eps, double weight_decay, const py::object& m_scales_, const py::object& v_scales_,
                 const std::optional<Tensor>& grad_scale, const std::optional<Tensor>& found_inf, const std::optional<Tensor>& grad_norm, const std::optional<Tensor>& grad_norm_wide,
                 double max_norm) {
+    const Tensors params(params_), m(m_), v(v_), steps(steps_);
+    Tensors grads(grads_);
+    std::optional<Tensors> m_scales, v_scales;
+    if (!m_scales_.is_none()) { m_scales.emplace(m_scales_); v_scales.emplace(v_scales_); }
     const bool eight = m_scales.has_value();
     const size_t n = params.size();
     for (const Tensors* l : {(const Tensors*)&grads, &m, &v, &steps, eight ? &*m_scales : &m, eight ? &*v_scales : &v})
@@ -164,7 +195,7 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& m, const Te
     for (size_t i = 0; i < n; ++i) {
         const bool dense = params[i].is_contiguous() && !params[i].is_neg() && m[i].is_contiguous() && v[i].is_contiguous() && (!eight || ((*m_scales)[i].is_contiguous() && (*v_scales)[i].is_contiguous()));
         refuse_unless(dense, "adamw_step: parameters and their state must be contiguous tensors");
-        if (!grads[i].is_contiguous() || grads[i].is_neg()) grads[i] = plain(grads[i]);
+        if (!grads[i].is_contiguous() || grads[i].is_neg()) grads.replace(i, plain(grads[i]));
         writes(steps[i]);
         if (!params[i].numel()) continue;      // (empty tensors have no address)
         writes(params[i]);
@@ -203,24 +234,25 @@ void adamw_step(const Tensors& params, Tensors grads, const Tensors& m, const Te
         check(api.adamw_step(&d, stream_of(dev)));
     }
     // written through raw pointers: whoever keys on a tensor's version has to see it
-    for (const Tensors* l : {&params, &m, &v, &steps, eight ? &*m_scales : nullptr, eight ? &*v_scales : nullptr})
+    for (const Tensors* l : {&params, &m, &v, &steps, eight ? (const Tensors*)&*m_scales : nullptr, eight ? (const Tensors*)&*v_scales : nullptr})
         if (l)
-            for (const Tensor& t : *l)
-                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            for (const Tensor* t : l->at)
+                if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
-std::pair<Tensor, Tensor> grad_norm(Tensors grads, const std::optional<Tensor>& grad_scale) {
-    refuse_unless(!grads.empty(), "grad_norm: no gradients");
+std::pair<Tensor, Tensor> grad_norm(const py::object& grads_, const std::optional<Tensor>& grad_scale) {
+    Tensors grads(grads_);
+    refuse_unless(grads.size(), "grad_norm: no gradients");
     strided("grad_norm", grads);
     const at::Device dev = grads[0].device();
-    for (const Tensor& g : grads) refuse_unless(dtype_of(g) >= 0, "grad_norm: gradients must be float32, bfloat16 or float16");
+    for (const Tensor* g : grads.at) refuse_unless(dtype_of(*g) >= 0, "grad_norm: gradients must be float32, bfloat16 or float16");
     same_device("grad_norm: the gradients", grads, dev);
     const c10::OptionalDeviceGuard guard(dev);
     std::vector<gf_norm_tensor_t> table;
     table.reserve(grads.size());
-    for (Tensor& g : grads) {
-        if (!g.is_contiguous() || g.is_neg()) g = plain(g);
-        table.push_back({g.data_ptr(), (uint64_t)g.numel(), (uint32_t)dtype_of(g), 0});
+    for (size_t i = 0; i < grads.size(); ++i) {
+        if (!grads[i].is_contiguous() || grads[i].is_neg()) grads.replace(i, plain(grads[i]));
+        table.push_back({grads[i].data_ptr(), (uint64_t)grads[i].numel(), (uint32_t)dtype_of(grads[i]), 0});
     }
     const Tensor out = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
     const Tensor work = at::empty({(int64_t)api.grad_norm_workspace_bytes((uint32_t)table.size())}, at::TensorOptions().dtype(at::kByte).device(dev));
