@@ -10,9 +10,11 @@ Per-model state (packed weights, fold matrices, workspace) is built once and cac
 import ctypes as C
 import itertools
 import random
+import weakref
 
 import numpy as np
 import torch
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from .lib import check, current_stream, lib, ptr
 
@@ -96,7 +98,7 @@ class FusedState:
 
         perm = (C.c_uint32 * 128)()
         check(L.gf_clayout_perm(perm))
-        self.perm = torch.tensor(list(perm), dtype=torch.long)
+        self.perm = torch.tensor(list(perm), dtype=torch.long).to(dev)
 
         a, s, c = model.ambient_net.net, model.sigma_net.net, model.color_net.net
         ind = _np(model.individual_embeddings[0]) if model.individual_embedding_dim > 0 else None
@@ -108,9 +110,9 @@ class FusedState:
         self._head_pack16 = None            # fast path: packed on first use (pack16)
         self._head_pack_split = None        # split path: packed on first use (pack_split)
         # ambient L1's cond_feat columns, rows in accumulator-layout order: amb_bias = W_cond @ cond_feat per frame
-        self.W_cond = a[0].weight.detach()[self.perm.to(dev), 32:].contiguous()
+        self.W_cond = a[0].weight.detach()[self.perm, 32:].contiguous()
         # colour L1's identity-code columns, same row order: col_bias = W_ind @ individual_code (field_forward with a per-call code)
-        self.W_ind = c[0].weight.detach()[self.perm.to(dev), 144:].contiguous() if model.individual_embedding_dim > 0 else None
+        self.W_ind = c[0].weight.detach()[self.perm, 144:].contiguous() if model.individual_embedding_dim > 0 else None
         if self.W_ind is not None:   # the folded identity-code bias is always this device product (refresh_weights computes the same one)
             off = int(L.gf_head_pack_colbias_offset())
             self.head_pack[off:off + 128] = torch.mv(self.W_ind, model.individual_embeddings[0].detach().float())
@@ -140,7 +142,7 @@ class FusedState:
                 check(L.gf_torso_pack(_hp(_np(d[0].weight)), _hp(_np(d[1].weight)), _hp(_np(d[2].weight)), _hp(_np(cn[0].weight)),
                                       _hp(_np(cn[1].weight)), _hp(_np(cn[2].weight)), _hp(tpack)))
             self.torso_pack = torch.from_numpy(tpack).to(dev)
-            p64, p32 = self.perm[:64].to(dev), self.perm[:32].to(dev)
+            p64, p32 = self.perm[:64], self.perm[:32]
             # per-frame constants [enc(pose) 54 | code 8] fold into the first-layer biases
             self.W_tconst = torch.cat([d[0].weight.detach()[p64, 42:], cn[0].weight.detach()[p32, 74:]], dim=0).contiguous()  # [96, 62]
             self.torso_S = float(np.log2(model.torso_embedder.per_level_scale))
@@ -150,6 +152,7 @@ class FusedState:
         # everything above is a COPY of (or a raw pointer into) model state: remember what it was built from (see get_state)
         self._watch = _watched_tensors(model)
         self.stamp = _stamp(self._watch)
+        _live.add(self)
 
     # ---- in-place weight updates (a training step, load_state_dict, a broadcast): repack on the device, no host round trip
     @staticmethod
@@ -190,7 +193,7 @@ class FusedState:
         flat = torch.cat([zero] + [w.detach().reshape(-1).float() for w in self._head_weights(model)])
         self.head_pack = flat[self._head_idx]
         a, c = model.ambient_net.net, model.color_net.net
-        perm = self.perm.to(dev)
+        perm = self.perm
         self.W_cond = a[0].weight.detach()[perm, 32:].contiguous()
         if model.individual_embedding_dim > 0:
             self.W_ind = c[0].weight.detach()[perm, 144:].contiguous()
@@ -339,6 +342,23 @@ def _watched_tensors(model):
 
 
 _untracked = itertools.count(-1, -1)
+_live = weakref.WeakSet()      # every FusedState in use
+
+
+def _after_optimizer_step(opt, args, kwargs):
+    """torch's fused optimizers (`fused=True`) write parameters without raising `_version`: raise it for those that a FusedState watches, or a
+    training step's forward pass would go on with the weights packed before the step."""
+    if not any(g.get("fused") for g in opt.param_groups):
+        return
+    watched = {id(t) for st in _live for t in st._watch}
+    for g in opt.param_groups:
+        if g.get("fused"):
+            for p in g["params"]:
+                if p.grad is not None and id(p) in watched and not p.is_inference():
+                    torch.autograd.graph.increment_version(p)
+
+
+register_optimizer_step_post_hook(_after_optimizer_step)
 
 
 def _ver(t) -> int:
