@@ -89,7 +89,7 @@ class _linear_tall(torch.autograd.Function):
 
 
 class MLP(nn.Module):
-    #: "native": torch's products in the layers' type; "fp8": both operands of every product in block-scaled 8 bits, added up in 32 (fp8.py), under
+    #: "native": torch's products in the layers' type; "fp8": both operands of every product in block-scaled 8 bits (fp8.py, also for how they are added up), under
     #: autograd and without it.  The stand-alone MLP and the op-by-op field (field_impl / render_impl "ops") go by it, the fused kernels do not.
     precision = "native"
 

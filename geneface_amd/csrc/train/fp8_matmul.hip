@@ -8,7 +8,6 @@
 #include "fp8_calls.hpp"
 #include "fp8_join.hpp"
 #include "geneface_train_hip.h"
-#include <type_traits>
 #include <utility>
 
 namespace gf {
@@ -61,9 +60,8 @@ constexpr int waitcnt(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 
 // Measured: m 8192, n 8192, k 4096 to bfloat16 in 222-250 us (2 200-2 480 TFLOP/s; the library's tensor-scaled product 226), 4096 each 58-65; to float32 (EXACT)
 // 4096 each 106-116 us (1 180-1 300 TFLOP/s).  The matrix units are busy for two thirds of a wave's life; the rest is the barrier of a step, first loads and last stores.
 //
-// EXACT: the 8-bit matrix instructions add the products of one instruction with about 17 bits (measured: 1.6e-5 of the result for normal values,
-// 5.6e-5 for log-normal ones, against 1e-7 of the bfloat16 instruction).  That is below half a step of a 16-bit result (2^-9, 2^-12), and not what a
-// 32-bit one should carry: for those the codes are widened to bfloat16 on the way out of LDS.
+// EXACT (kExact<T>): codes are widened to bfloat16 on the way out of LDS and added up on its instruction, in 32 bits.  8192 x 8192 x 4096 to binary16 takes
+// 403 us that way, 222 on the 8-bit instruction; 333 rows, 8192 -> 2048 29.5 for 22.4; a few rows 5.8 for 5.4.
 template <typename T, bool EXACT, int TM, int TN, int STAGES>
 __device__ __forceinline__ void matmul_tile(const MatmulArgs& d, const uint32_t block, const uint32_t split) {
     constexpr int BM = 64 * TM, BN = 64 * TN, LA = BM / 32, LB = BN / 32;      // 32 rows of 128 bytes a load of the workgroup
@@ -285,8 +283,8 @@ template <typename A, typename B>
 __global__ __launch_bounds__(256) void k_matmul_two(const MatmulArgs a, const MatmulArgs b) {
 #ifdef __HIP_DEVICE_COMPILE__      // (the host's pass finds no candidate for these calls, and has no use for them)
     const uint32_t tiles = a.tiles_m * a.tiles_n, first = (tiles + 7) & ~7u;
-    if (blockIdx.x >= first) matmul_tile<B, sizeof(B) == 4, 1, 1, 4>(b, blockIdx.x - first, 0);
-    else if (blockIdx.x < tiles) matmul_tile<A, sizeof(A) == 4, 1, 1, 4>(a, blockIdx.x, 0);
+    if (blockIdx.x >= first) matmul_tile<B, kExact<B>, 1, 1, 4>(b, blockIdx.x - first, 0);
+    else if (blockIdx.x < tiles) matmul_tile<A, kExact<A>, 1, 1, 4>(a, blockIdx.x, 0);
 #endif
 }
 
@@ -347,7 +345,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d) 
                 if (b >= here) break;
                 const i32x4 xl = *reinterpret_cast<const i32x4*>(codes + xr * pitch + b * 128 + q * 32), xh = *reinterpret_cast<const i32x4*>(codes + xr * pitch + b * 128 + q * 32 + 16);
                 const uint32_t sx = bytes[xr * here + b];
-                if constexpr (sizeof(T) == 4) {      // a 32-bit result: see EXACT above
+                if constexpr (kExact<T>) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const i32x4 pw = i < 2 ? lo[u] : hi[u], px = i < 2 ? xl : xh;
@@ -373,8 +371,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_rows(const gf_fp8_rows_t d) 
 }
 
 // The tile and how many ways the sum over K is split: the choice with the least time of its longest CU, in units of 0.11 us.  A workgroup's step over
-// one block takes 2 of them for a tile of 64 x 64, 3 for 128 x 64, 5 for 128 x 128 and 17 for 256 x 256 (about 1.7 times that each for the 32-bit
-// result): large tiles read less per product, small ones give every CU one (the three small tiles all read some 32 bytes a clock and CU, which is what
+// one block takes 2 of them for a tile of 64 x 64, 3 for 128 x 64, 5 for 128 x 128 and 17 for 256 x 256 (about 1.7 times that each for EXACT
+// ones): large tiles read less per product, small ones give every CU one (the three small tiles all read some 32 bytes a clock and CU, which is what
 // bounds them; fragments straight from memory to registers, without LDS, read half of that).  A split's parts cost 45, their launch among it, and the way to memory and
 // back.  Measured, us, 64 x 64 / 128 x 64 / 128 x 128 / 256 x 256: m 333, n 2048, k 8192 16.9 / 21 / 22 / -, split in two 128 x 64 18.3, in four
 // 128 x 128 18.1; 512, 4096, 4096 16.6 / 13.7 / 17.1 / -; 2048 each 17.7 / 15.9 / 13.8 / 25.5; 4096 each 111 / 103 / 70 / 62.
@@ -413,7 +411,7 @@ static void launch_tiles(const MatmulArgs& a, const Plan& p, hipStream_t s) {
 
 template <typename T>
 static void launch_matmul(MatmulArgs a, const Plan& p, void* workspace, hipStream_t s) {
-    constexpr bool exact = sizeof(T) == 4;
+    constexpr bool exact = kExact<T>;
     if (p.splits == 1) { launch_tiles<T, exact>(a, p, s); return; }
     T* out = (T*)a.out;
     a.out = workspace;

@@ -28,7 +28,7 @@ __device__ __forceinline__ i32x8 fragment(const uint8_t* tile, int r, int half, 
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// acc += a b^T over half a block; 32-bit results on the bfloat16 instruction (fp8_matmul.hip, EXACT)
+// acc += a b^T over half a block
 template <bool EXACT>
 __device__ __forceinline__ f32x16 multiply_half(i32x8 a, i32x8 b, f32x16 acc, uint32_t sa, uint32_t sb) {
     if constexpr (EXACT) {
@@ -128,8 +128,8 @@ __device__ __forceinline__ void rows_product(uint8_t* codes, const uint8_t* scal
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
         const int r = k * 32 + (lane & 31);
-        acc = multiply_half<sizeof(T) == 4>(fragment(other, r, 0, lane), x0, acc, other_scale, sx);
-        acc = multiply_half<sizeof(T) == 4>(fragment(other, r, 1, lane), x1, acc, other_scale, sx);
+        acc = multiply_half<kExact<T>>(fragment(other, r, 0, lane), x0, acc, other_scale, sx);
+        acc = multiply_half<kExact<T>>(fragment(other, r, 1, lane), x1, acc, other_scale, sx);
         // 32 x 32 results through LDS, so that a row's 128 (64) bytes leave together
         __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_wave_barrier();

@@ -1,7 +1,7 @@
 """Linear products of block-scaled 8-bit values, with their gradients.
 
 The arithmetic of `cond_encoder.MLP`'s bias-free layers (cond_encoder.py:92-111 of the reference) with both operands of every product brought to e4m3 in
-blocks of 128 along the axis that is summed over, and added up in 32 bits:
+blocks of 128 along the axis that is summed over, and added up in 32 bits (bfloat16 results: see `linear`):
 
     y  = Q_row(x)  Q_tile(W)^T        dx = Q_row(dy) Q_tile(W)        dW = Q_col(dy)^T Q_col(x)
 
@@ -129,8 +129,12 @@ def linear(x, weight):
 
     weight: a tensor [N, K], quantised in the call, with gradients to x and to the weight; or an Fp8Weight, without gradients.  x, weight: float32,
     bfloat16 or float16, each its own; the gradients have their input's type.  At most 8388480 values along each sum, unless both of the weight's
-    sides are 128 or less.  Results of 16 bits are added up on the 8-bit matrix instructions (about 17 bits within one instruction, 32 between
-    them), results of 32 bits in 32.
+    sides are 128 or less.
+
+    float32 and binary16 results (y and dx in x's type, dw in the weight's) are added up in 32 bits.  bfloat16 results come from the 8-bit matrix
+    instructions, which line up the products of eight neighbours along the sum and drop what lies below 2^-13 of the largest: a sum loses at most
+    7 * 2^-13 of each eight's largest product (8.5e-4, where bfloat16 rounds by 3.9e-3; normal operands: 2.5e-6), whatever its length.
+    For less, give x (or the weight, for dw) in float32.
 
     Both directions may be captured into a graph.  As with any torch node, a backward pass is captured only while no graph of the same leaves lives
     that was built outside the capture.  Gradients of the gradients are refused."""

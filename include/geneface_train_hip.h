@@ -82,7 +82,8 @@ int gf_grad_norm(const gf_grad_norm_t* desc, void* stream);
  *
  * Codes are e4m3 (largest 448).  A block of 128 values has the scale 2^(byte - 127): the smallest power of two >= 2^-127 with
  * (largest magnitude) <= 448 * scale; the byte is 255 and every code NaN where the block holds an infinity or a NaN.  Codes are
- * rounded to nearest even.  An operand [R, K] that is summed over K is held as codes [R, Kp], Kp = K rounded up to a multiple of 128 and the
+ * rounded to nearest even.  Products are added up in 32 bits where the result is float32 or binary16; where it is bfloat16, products of eight neighbours
+ * along the sum are first added with what each has above 2^-13 of the largest of them (at most 7 * 2^-13 of that is lost), the eights in 32 bits.  An operand [R, K] that is summed over K is held as codes [R, Kp], Kp = K rounded up to a multiple of 128 and the
  * codes behind K zero, and scales either by row, byte (r, b) at [b * pitch + r], or by tile of 128 x 128, byte at [(r / 128) * stride_row + b *
  * stride_block].
  * ---------------------------------------------------------------------------------------------- */
@@ -112,7 +113,7 @@ typedef struct {
     uint64_t stride_row, stride_block;
 } gf_fp8_operand_t;
 
-/* out [m, n] of `dtype` (contiguous) = a [m, 128 blocks] b [n, 128 blocks]^T, added up in 32 bits; blocks <= 65535.
+/* out [m, n] of `dtype` (contiguous) = a [m, 128 blocks] b [n, 128 blocks]^T; blocks <= 65535.
  * workspace: gf_fp8_matmul_workspace_bytes(m, n, blocks) device bytes of this call's own (NULL where that is 0). */
 typedef struct {
     gf_fp8_operand_t a, b;
