@@ -193,6 +193,21 @@ __device__ __forceinline__ void step8(const gf_adamw_tensor_t& t, const Hyper& h
             am = max_abs(am, fm[k]);
             ar = max_abs(ar, fr[k]);
         }
+        // A root whose square leaves the type's range: a gradient above 1.8e19 / sqrt(1 - beta2), or a root above 1.8e19 that is still held.  The root itself does
+        // not, and an infinite one would freeze all 128 values for good: it is formed again from what is still in memory, scaled.
+        if (ar == __builtin_inff()) {
+            ar = 0;
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k) {
+                if (fr[k] == __builtin_inff() && __builtin_fabsf(fm[k]) < __builtin_inff() && (k & 3) < left[k >> 2]) {
+                    const uint64_t i = i0 + 64 * (k >> 2) + (k & 3);
+                    const float r = __builtin_amdgcn_cvt_f32_fp8((int)v[i], 0) * vs * 0x1p-66f, x = (float)g[i] * h.grad * 0x1p-66f;
+                    fr[k] = fminf(sqrtf(moment2(h, r * r, x)) * 0x1p66f, 3.4028234663852886e38f);
+                    fp[k] = updated(h, (float)p[i], fm[k], fr[k]);
+                }
+                ar = max_abs(ar, fr[k]);
+            }
+        }
         // as integers: what is no number stays the largest and makes the whole block none
         const uint32_t bm = row_max_u32(__float_as_uint(am)), br = row_max_u32(__float_as_uint(ar));
         const float a_m = max_abs(kTiny, __uint_as_float(bm)), a_r = max_abs(kTiny, __uint_as_float(br));

@@ -7,7 +7,8 @@ it.  With `weight_decay=0` it is Adam.
 8-bit moments: e4m3 codes with one 32-bit scale for each 128 consecutive values of a tensor, max(largest magnitude, 2^-100) times 1 / 448.  The second
 moment is held as its square root, which halves the range it needs.  Codes are rounded by a dither that depends on the step and on the value's
 index only, so a step is reproducible and changes far below the format's spacing add up over the steps; a second moment above zero is never rounded
-to zero.  A block that meets a gradient that is no finite number is none afterwards (all 128 values).
+to zero.  Held as its root it does not overflow either: any finite gradient leaves a finite one (in 32 bits, as in torch.optim.AdamW, a gradient above
+1.8e19 / sqrt(1 - beta2) leaves an infinite one, and its parameter stands still from then on).  A block that meets a gradient that is no finite number is none afterwards (all 128 values).
 
 Everything is done on the current stream of the tensors' device and may be captured into a graph; a graph keeps the addresses, and numbers given
 as Python numbers (`lr` as a one-element tensor on the device stays adjustable).
