@@ -88,9 +88,15 @@ class _linear_tall(torch.autograd.Function):
         return gx, gw
 
 
+def all_native(model):
+    """Whether every MLP of a model computes in its layers' type, as the fused kernels do."""
+    return all(getattr(m, "precision", "native") == "native" for m in model.children())
+
+
 class MLP(nn.Module):
     #: "native": torch's products in the layers' type; "fp8": both operands of every product in block-scaled 8 bits (fp8.py, also for how they are added up), under
-    #: autograd and without it.  The stand-alone MLP and the op-by-op field (field_impl / render_impl "ops") go by it, the fused kernels do not.
+    #: autograd and without it.  The fused kernels have no such form: a model one of whose MLPs is not "native" takes the op-by-op field where its
+    #: field_impl / render_impl is "auto", and refuses "fused".
     precision = "native"
 
     def __init__(self, dim_in, dim_out, dim_hidden, num_layers):

@@ -16,6 +16,7 @@ import numpy as np
 import torch
 from torch.optim.optimizer import register_optimizer_step_post_hook
 
+from .cond_encoder import all_native
 from .lib import check, current_stream, lib, ptr
 
 _u32, _f32, _vp = C.c_uint32, C.c_float, C.c_void_p
@@ -384,6 +385,8 @@ def get_state(model) -> FusedState:
     if torch.is_autocast_enabled():
         with torch.autocast("cuda", enabled=False):
             return get_state(model)
+    if not all_native(model):
+        raise NotImplementedError("fused path: an MLP's precision is not 'native' (use render_impl='ops' or 'auto')")
     st = getattr(model, "_fused_state", None)
     if st is None or st.device != model.density_bitfield.device:
         st = FusedState(model)

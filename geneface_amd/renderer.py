@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 
 from . import raymarching
+from .cond_encoder import all_native
 
 
 def _rand_like(x, generator=None):
@@ -244,6 +245,8 @@ class NeRFRenderer(nn.Module):
     def _pick_impl(self, impl, perturb, max_steps):
         if impl != "auto":
             return impl
+        if not all_native(self):
+            return "ops"
         if max_steps > 1024:      # beyond the reference's own default and viewer maximum (renderer.py:263, radnerf_gui.py:466-471)
             return "ops"
         ok = getattr(self, "_fused_arch_ok", None)
