@@ -131,8 +131,6 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, varia
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         host = ex.submit(build_host, force) if not tag else None
         results = list(ex.map(lambda s: _compile(s, force, extra, obj_dir, tuple(drop_flags)), [*sources(), *train_sources()]))
-        if host is not None:
-            host.result()
     objs = [o for o, _ in results]
     if force or any(ch for _, ch in results) or not os.path.exists(out):
         cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *objs, "-o", out, "-lz", "-lpthread"]   # zlib: the PNG frame writer (png_writer.cpp)
@@ -141,6 +139,8 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, varia
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         if verbose:
             print("linked", out)
+    if host is not None and host.exception() is not None:      # the C ABI needs neither g++ nor Python's and torch's headers: lib.host() says what is missing when it is asked for
+        sys.stderr.write(f"geneface_amd: {out} is built, the Python side of the training operators is not: {host.exception()}\n")
     return out
 
 

@@ -1,0 +1,41 @@
+"""The build's steps with stand-in compilers: what fails, and what is left on the disk then."""
+import os
+import stat
+
+import pytest
+
+from geneface_amd.csrc import build
+
+
+def _compiler(path, body):
+    """A program that finds the file behind -o as $out."""
+    path.write_text('#!/bin/sh\nwhile [ $# -gt 0 ]; do [ "$1" = -o ] && out=$2; shift; done\n' + body + "\n")
+    path.chmod(path.stat().st_mode | stat.S_IXUSR)
+    return str(path)
+
+
+@pytest.fixture
+def places(tmp_path, monkeypatch):
+    """Everything that is built goes to a folder of the test's own, compilers come from there."""
+    monkeypatch.setattr(build, "OUT", str(tmp_path / "lib.so"))
+    monkeypatch.setattr(build, "HOST_OUT", str(tmp_path / "host.so"))
+    monkeypatch.setattr(build, "OBJ_DIR", str(tmp_path / "obj"))
+    monkeypatch.setattr(build, "HIPCC", _compiler(tmp_path / "hipcc", 'echo made > "$out"'))
+    monkeypatch.setenv("PATH", str(tmp_path) + os.pathsep + os.environ["PATH"])
+    return tmp_path
+
+
+def test_the_library_needs_no_host_compiler(places, capsys):
+    _compiler(places / "g++", "echo no such header >&2; exit 1")
+    assert build.build() == str(places / "lib.so") and (places / "lib.so").read_text() == "made\n"
+    assert "no such header" in capsys.readouterr().err
+    with pytest.raises(RuntimeError, match="no such header"):
+        build.build_host()
+
+
+def test_a_failing_device_compiler_is_an_error(places):
+    _compiler(places / "g++", 'echo made > "$out"')
+    _compiler(places / "hipcc", "echo wrong >&2; exit 1")
+    with pytest.raises(RuntimeError, match="wrong"):
+        build.build()
+    assert not (places / "lib.so").exists()
