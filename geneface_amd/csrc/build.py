@@ -76,6 +76,20 @@ def source_digest() -> str:
     return h.hexdigest()[:16]
 
 
+def _run(cmd, out, what):
+    """Run a compiler with `-o out`, completely or not at all: other processes (ranks that start together) load and link what lies at `out`."""
+    part = f"{out}.{os.getpid()}.part"
+    try:
+        r = subprocess.run([*cmd, "-o", part], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"{what}:\n{r.stdout}\n{r.stderr}")
+        os.replace(part, out)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+    return r
+
+
 def _compile(src, force, extra=(), obj_dir=OBJ_DIR, drop=()):
     obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
     train = os.path.dirname(src) == TRAIN_DIR
@@ -86,11 +100,9 @@ def _compile(src, force, extra=(), obj_dir=OBJ_DIR, drop=()):
     newest = max(os.path.getmtime(p) for p in [src, __file__, *(train_headers() if train else headers())])
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= newest:
         return obj, False
-    cmd = [HIPCC, *[f for f in COMMON if f not in drop], *PER_FILE.get(os.path.basename(src), ()), *extra, "-x", "hip", "-c", src, "-o", obj, "-I", HERE,
+    cmd = [HIPCC, *[f for f in COMMON if f not in drop], *PER_FILE.get(os.path.basename(src), ()), *extra, "-x", "hip", "-c", src, "-I", HERE,
            "-I", os.path.join(HERE, "..", "..", "include")]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
+    r = _run(cmd, obj, f"hipcc failed for {src}")
     said = "".join(line for line in r.stderr.splitlines(True) if "packed-fp32-ops" not in line)      # the host pass does not know the feature
     if said.strip():
         sys.stderr.write(said)
@@ -109,10 +121,8 @@ def build_host(force: bool = False) -> str:
            "/opt/rocm/include", os.path.join(HERE, "..", "..", "include")]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_train_host", *[f"-I{i}" for i in inc], HOST_SOURCE,
-           "-o", HOST_OUT, f"-L{os.path.join(home, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {HOST_SOURCE}:\n{r.stdout}\n{r.stderr}")
+           f"-L{os.path.join(home, 'lib')}", "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
+    _run(cmd, HOST_OUT, f"g++ failed for {HOST_SOURCE}")
     return HOST_OUT
 
 
@@ -133,10 +143,8 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, varia
         results = list(ex.map(lambda s: _compile(s, force, extra, obj_dir, tuple(drop_flags)), [*sources(), *train_sources()]))
     objs = [o for o, _ in results]
     if force or any(ch for _, ch in results) or not os.path.exists(out):
-        cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *objs, "-o", out, "-lz", "-lpthread"]   # zlib: the PNG frame writer (png_writer.cpp)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+        cmd = [HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *objs, "-lz", "-lpthread"]   # zlib: the PNG frame writer (png_writer.cpp)
+        _run(cmd, out, "link failed")
         if verbose:
             print("linked", out)
     if host is not None and host.exception() is not None:      # the C ABI needs neither g++ nor Python's and torch's headers: lib.host() says what is missing when it is asked for

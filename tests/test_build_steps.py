@@ -39,3 +39,29 @@ def test_a_failing_device_compiler_is_an_error(places):
     with pytest.raises(RuntimeError, match="wrong"):
         build.build()
     assert not (places / "lib.so").exists()
+
+
+def test_nothing_half_written_is_left_where_others_look(places):
+    """A compiler that dies while it writes: what was there before is still there, whole, and no piece of a file beside it."""
+    good, half = 'echo made > "$out"', 'echo half > "$out"; exit 1'
+    _compiler(places / "g++", good)
+    build.build()
+    before = {f: f.read_text() for f in places.rglob("*") if f.suffix in (".so", ".o")}
+    assert len(before) > 10 and set(before.values()) == {"made\n"}
+    _compiler(places / "g++", half)
+    with pytest.raises(RuntimeError):
+        build.build_host(force=True)
+    _compiler(places / "hipcc", half)
+    with pytest.raises(RuntimeError):
+        build.build(force=True)
+    _compiler(places / "hipcc", f'case "$out" in *lib.so*) {half};; *) {good};; esac')
+    with pytest.raises(RuntimeError):
+        build.build(force=True)
+    assert {f: f.read_text() for f in places.rglob("*") if f.suffix in (".so", ".o")} == before
+    assert not [f for f in places.rglob("*") if "half" in f.name or f.name.endswith(".part")]
+
+
+def test_a_file_appears_when_it_is_whole(places):
+    """While the compiler writes, nothing is there to be loaded."""
+    _compiler(places / "g++", f'echo half > "$out"; [ -e {places / "host.so"} ] && echo early >&2 && exit 1; echo whole >> "$out"')
+    assert build.build_host() == str(places / "host.so") and (places / "host.so").read_text() == "half\nwhole\n"
