@@ -148,8 +148,9 @@ template <typename T> constexpr bool kExact = !std::is_same<T, __bf16>::value;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// Sixteen codes' products at a time on the bfloat16 matrix instruction, with the blocks' scales multiplied in: exact, since a code has four
-// significant bits and a scale none.
+// Sixteen codes' products at a time on the bfloat16 matrix instruction, with the blocks' scales multiplied in: exact where the scale is 2^-124 or more, since a
+// code has four significant bits and a scale none.  Below, values are rounded to bfloat16's last step of 2^-133: a sum is off by at most 2^-134 times the
+// other operand's magnitudes.
 __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float scale) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
     const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
