@@ -1,9 +1,13 @@
 """GPU: a model's MLPs in 8 bits are computed in 8 bits whichever way the model is called, and beside the native ones within what 8 bits round."""
 import copy
+import math
 
 import pytest
 import torch
 
+import fp8_reference as R
+from geneface_amd import fp8, optim
+from geneface_amd.cond_encoder import MLP
 from helpers import frame_inputs, model_fixture, sequence
 
 pytestmark = pytest.mark.gpu
@@ -60,3 +64,69 @@ def test_rendering_goes_by_it_or_refuses(torso):
         with pytest.raises(NotImplementedError, match="precision"):
             run("fused")
 
+
+class _Formula(torch.autograd.Function):
+    """A layer and its gradients from the format's definition, added up in 64 bits."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        ctx.save_for_backward(x, w)
+        return (R.by_rows(x) @ R.by_tiles(w).t()).float().to(x.device)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        return (R.by_rows(dy) @ R.by_tiles(w)).float().to(x.device), (R.by_columns(dy).t() @ R.by_columns(x)).float().to(x.device)
+
+
+def test_field_in_8_bits_is_the_formula(monkeypatch):
+    """Density, colour and every gradient of the model against the same model with its layers from the definition.  Sums in 32 and in 64 bits differ by some 1e-6,
+    which moves one code in ten thousand to its neighbour, 6 % away: some 1e-3 of a layer's norm at most, over eight layers and the tables below 1e-2."""
+    _, model = _model()
+    model.train()
+    for m in (model.ambient_net, model.sigma_net, model.color_net):
+        m.precision = "fp8"
+    pos, dirs, cond = _points(1500)
+    cond.requires_grad_(True)
+
+    def run():
+        model.zero_grad(set_to_none=True)
+        cond.grad = None
+        sigma, rgb, amb = model(pos, dirs, cond, model.individual_embeddings[0])
+        ((sigma.clamp(max=50) * 0.1).mean() + rgb.square().mean() + amb.square().mean()).backward()
+        out = {"sigma": sigma, "rgb": rgb, "ambient": amb, "d cond": cond.grad, **{"d " + n: p.grad for n, p in model.named_parameters() if p.grad is not None}}
+        return {k: v.detach().double().clone() for k, v in out.items()}
+    ours = run()
+    monkeypatch.setattr(fp8, "linear", _Formula.apply)
+    want = run()
+    assert set(ours) == set(want) and len([k for k in ours if "_net.net" in k]) == 8
+    for k, v in want.items():
+        assert float(v.norm()) > 0 and float((ours[k] - v).norm() / v.norm()) < 1e-2, (k, float((ours[k] - v).norm() / v.norm()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_step_of_an_mlp_is_clipped(bits):
+    """The moments after the first step are those of the clipped gradients: exact to eight roundings in 32 bits, to one spacing of their codes in 8."""
+    torch.manual_seed(3)
+    net = MLP(96, 3, 128, 3).cuda()
+    net.precision = "fp8"
+    b1, b2 = 0.9, 0.99
+    opt = optim.AdamW(net.parameters(), lr=1e-2, betas=(b1, b2), eps=1e-15, state_bits=bits, max_grad_norm=1.0)
+    scaler = torch.amp.GradScaler("cuda", init_scale=256.0)
+    x = torch.randn(2000, 96, generator=torch.Generator().manual_seed(1)).cuda()
+    scaler.scale(net(x).square().mean()).backward()
+    grads = [p.grad.double() / 256 for p in net.parameters()]
+    norm = math.sqrt(sum(float(v.pow(2).sum()) for v in grads))
+    opt.max_grad_norm = 0.25 * norm
+    c = 0.25 * norm / (norm + 1e-6)
+    scaler.step(opt)
+    assert abs(float(opt.last_grad_norm) - norm) <= 2.0 ** -23 * norm
+    for p, g in zip(net.parameters(), grads):
+        m, v = (t.double() for t in opt.moments(p))
+        for got, want in ((m, (1 - b1) * c * g), (v.sqrt(), math.sqrt(1 - b2) * c * g.abs())):
+            spacing = 8 * 2.0 ** -24 * want.abs()
+            if bits == 8:
+                least = torch.nn.functional.pad(want.abs().flatten(), (0, -want.numel() % 128)).view(-1, 128).amax(1, keepdim=True).clamp(min=2.0 ** -100) / 448 * 2.0 ** -9
+                least = least.expand(-1, 128).flatten()[:want.numel()].view(want.shape)
+                spacing = (2.0 ** -3 * want.abs()).clamp(min=least) * (1 + 2.0 ** -20)
+            assert bool(((got - want).abs() <= spacing).all())
