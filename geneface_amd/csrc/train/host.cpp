@@ -145,6 +145,12 @@ void sort_by_address(std::vector<Span>& spans) {
     }
 }
 
+// Whether anything of [first, behind) is among the sorted spans, which do not overlap.
+bool touches(const std::vector<Span>& spans, uintptr_t first, uintptr_t behind) {
+    const auto next = std::upper_bound(spans.begin(), spans.end(), first, [](uintptr_t a, const Span& s) { return a < s.behind; });      // the first that ends behind `first`
+    return next != spans.end() && next->first < behind;
+}
+
 // ---- AdamW ---------------------------------------------------------------------------------------------------------------------------------
 
 void adamw_step(const py::object& params_, const py::object& grads_, const py::object& m_, const py::object& v_, const py::object& steps_, double lr,
@@ -209,6 +215,14 @@ void adamw_step(const py::object& params_, const py::object& grads_, const py::o
     sort_by_address(written);
     for (size_t i = 1; i < written.size(); ++i)
         refuse_unless(written[i - 1].behind <= written[i].first, "adamw_step: the same tensor is given twice, or two that share memory");
+    auto reads = [&](const void* p, size_t bytes) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+        refuse_unless(!bytes || !touches(written, at, at + bytes), "adamw_step: a gradient or a scalar shares memory with what the step writes");
+    };
+    for (size_t i = 0; i < n; ++i)      // (a gradient that is its own parameter is read where it is written, by the same thread)
+        if (grads[i].data_ptr() != params[i].data_ptr()) reads(grads[i].data_ptr(), grads[i].nbytes());
+    for (const std::optional<Tensor>* t : {&lr_device, &grad_scale, &found_inf, &grad_norm, &grad_norm_wide})
+        if (*t) reads((*t)->data_ptr(), (*t)->nbytes());
     gf_adamw_t d = {};
     d.state_bits = eight ? 8 : 32;
     d.lr = lr; d.beta1 = beta1; d.beta2 = beta2; d.eps = eps; d.weight_decay = weight_decay; d.max_norm = max_norm;

@@ -55,7 +55,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
 
     params, grads: float32, bfloat16 or float16, gradients of their parameter's type and size.  exp_avgs, exp_avg_sqs: float32 of the same sizes,
     or -- with exp_avg_scales and exp_avg_sq_scales, lists of float32 [ceil(numel / 128)] -- float8_e4m3fn.  steps: one float32 each, the number of
-    steps taken so far.  Everything on one device; all but gradients must be contiguous, and no two of them may share memory.
+    steps taken so far.  Everything on one device; all but gradients must be contiguous.  What is written shares memory with
+    nothing else that is given (a gradient may be its own parameter).
 
     lr: a number, or one float32 on the device.  grad_scale: the factor that the gradients carry.  found_inf: where it is not 0 nothing is
     changed, the step counts included.  grad_norm, max_norm: gradients are multiplied by min(1, max_norm / (grad_norm + 1e-6)); both or neither.

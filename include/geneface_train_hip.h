@@ -35,7 +35,7 @@ typedef struct {
 /* Host descriptor; tensors_host is read during the call.  grad_scale, found_inf, grad_norm and lr_device are one float on the device each, or
  * NULL.  The gradients that enter are g / grad_scale min(1, max_norm / (grad_norm + 1e-6)); grad_norm_wide:
  * the norm in 64 bits, taken where it rounds to *grad_norm, or NULL.  Where *found_inf is not 0 nothing is changed, the
- * step counts included.  lr_device replaces lr.  dtype: of p and g.  state_bits: 32 or 8. */
+ * step counts included.  What is written is read through no other pointer; g may be its own p.  lr_device replaces lr.  dtype: of p and g.  state_bits: 32 or 8. */
 typedef struct {
     const gf_adamw_tensor_t* tensors_host;
     uint32_t count;
