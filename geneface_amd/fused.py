@@ -84,6 +84,17 @@ def _pack_index(pack, shapes, n_out):
     return torch.from_numpy(idx)
 
 
+_PACK_INDEX = {}
+
+
+def _pack_index_on(dev, pack, shapes, n_out):
+    """_pack_index on a device, made once for a layout: a FusedState lives from one occupancy update to the next, its maps are the same every time."""
+    key = (str(dev), *shapes, n_out)
+    if key not in _PACK_INDEX:
+        _PACK_INDEX[key] = _pack_index(pack, shapes, n_out).to(dev)
+    return _PACK_INDEX[key]
+
+
 class FusedState:
     """Everything the kernels need that depends only on the model (built once, device resident)."""
 
@@ -153,6 +164,8 @@ class FusedState:
         # everything above is a COPY of (or a raw pointer into) model state: remember what it was built from (see get_state)
         self._watch = _watched_tensors(model)
         self.stamp = _stamp(self._watch)
+        # which of them only the torso's packs are made of
+        self._torso_only = {i for i, (n, _) in enumerate(model.named_parameters()) if n.startswith(("torso", "head_color_weights_encoder"))}
         _live.add(self)
 
     # ---- in-place weight updates (a training step, load_state_dict, a broadcast): repack on the device, no host round trip
@@ -181,14 +194,26 @@ class FusedState:
             e0 = model.head_color_weights_encoder(torch.zeros(1, 4, device=self.device)).reshape(-1).float()
         return torch.cat([code, e0]).contiguous(), torch.cat([code, torch.zeros_like(e0)]).contiguous()
 
-    def refresh_weights(self, model):
-        """The packed copies follow the model's current weights: per pack one cat + one gather on the device."""
+    def refresh_weights(self, model, head=True, torso=True):
+        """The packed copies follow the model's current weights: per pack one cat + one gather on the device.  head / torso: which of them changed (a torso is
+        trained beside a head that is not)."""
+        if head:
+            self._refresh_head(model)
+        if torso and self.has_torso:
+            self._refresh_torso(model)
+        if self.cond is not None:          # the cached gf_cond_t points at W_cond / W_tconst / the torso code
+            self.cond.W_cond = ptr(self.W_cond)
+            if self.has_torso:
+                self.cond.W_tconst = ptr(self.W_tconst)
+                self.cond.torso_code = ptr(self._torso_code) if self._torso_code is not None else None
+
+    def _refresh_head(self, model):
         L = lib()
         dev = self.device
         if self._head_idx is None:
             ws = self._head_weights(model)
-            self._head_idx = _pack_index(lambda arr, out: check(L.gf_head_pack(*[_hp(a) for a in arr], None, _hp(out))),
-                                         [tuple(w.shape) for w in ws], L.gf_head_pack_floats()).to(dev)
+            self._head_idx = _pack_index_on(dev, lambda arr, out: check(L.gf_head_pack(*[_hp(a) for a in arr], None, _hp(out))),
+                                            [tuple(w.shape) for w in ws], L.gf_head_pack_floats())
             self._colbias_off = int(L.gf_head_pack_colbias_offset())
         zero = torch.zeros(1, dtype=torch.float32, device=dev)
         flat = torch.cat([zero] + [w.detach().reshape(-1).float() for w in self._head_weights(model)])
@@ -200,29 +225,28 @@ class FusedState:
             self.W_ind = c[0].weight.detach()[perm, 144:].contiguous()
             self.head_pack[self._colbias_off:self._colbias_off + 128] = torch.mv(self.W_ind, model.individual_embeddings[0].detach().float())
         self._head_pack16 = self._head_pack_split = None
-        if self.has_torso:
-            n_main = L.gf_torso_pack_floats()
-            if self._torso_idx is None:
-                ws = self._torso_weights(model)
-                if self.head_aware:
-                    packer = lambda arr, out: check(L.gf_torso_pack_ha(*[_hp(a) for a in arr], _hp(out[:n_main]), _hp(out[n_main:])))
-                    n_out = n_main + L.gf_torso_ha_pack_floats()
-                else:
-                    packer, n_out = (lambda arr, out: check(L.gf_torso_pack(*[_hp(a) for a in arr], _hp(out)))), n_main
-                self._torso_idx = _pack_index(packer, [tuple(w.shape) for w in ws], n_out).to(dev)
-            flat = torch.cat([zero] + [w.detach().reshape(-1).float() for w in self._torso_weights(model)])
-            both = flat[self._torso_idx]
-            self.torso_pack = both[:n_main].contiguous()
+
+    def _refresh_torso(self, model):
+        L = lib()
+        dev = self.device
+        n_main = L.gf_torso_pack_floats()
+        if self._torso_idx is None:
+            ws = self._torso_weights(model)
             if self.head_aware:
-                self.torso_ha_pack = both[n_main:].contiguous()
-            d, cn = model.torso_deform_net.net, model.torso_canonicial_net.net
-            self.W_tconst = torch.cat([d[0].weight.detach()[perm[:64], 42:], cn[0].weight.detach()[perm[:32], 74:]], dim=0).contiguous()
-            self._torso_code, self._torso_code_ha = self._torso_codes(model)
-        if self.cond is not None:          # the cached gf_cond_t points at W_cond / W_tconst / the torso code
-            self.cond.W_cond = ptr(self.W_cond)
-            if self.has_torso:
-                self.cond.W_tconst = ptr(self.W_tconst)
-                self.cond.torso_code = ptr(self._torso_code) if self._torso_code is not None else None
+                packer = lambda arr, out: check(L.gf_torso_pack_ha(*[_hp(a) for a in arr], _hp(out[:n_main]), _hp(out[n_main:])))
+                n_out = n_main + L.gf_torso_ha_pack_floats()
+            else:
+                packer, n_out = (lambda arr, out: check(L.gf_torso_pack(*[_hp(a) for a in arr], _hp(out)))), n_main
+            self._torso_idx = _pack_index_on(dev, packer, [tuple(w.shape) for w in ws], n_out)
+        zero = torch.zeros(1, dtype=torch.float32, device=dev)
+        flat = torch.cat([zero] + [w.detach().reshape(-1).float() for w in self._torso_weights(model)])
+        both = flat[self._torso_idx]
+        self.torso_pack = both[:n_main].contiguous()
+        if self.head_aware:
+            self.torso_ha_pack = both[n_main:].contiguous()
+        d, cn = model.torso_deform_net.net, model.torso_canonicial_net.net
+        self.W_tconst = torch.cat([d[0].weight.detach()[self.perm[:64], 42:], cn[0].weight.detach()[self.perm[:32], 74:]], dim=0).contiguous()
+        self._torso_code, self._torso_code_ha = self._torso_codes(model)
 
     def refresh_occupancy(self, model):
         bits = np.ascontiguousarray(model.density_bitfield.detach().cpu().numpy().astype(np.uint8))
@@ -402,7 +426,8 @@ def get_state(model) -> FusedState:
         if stamp[n_param:] != st.stamp[n_param:]:                       # an occupancy buffer changed in place
             st.refresh_occupancy(model)
         if stamp[:n_param] != st.stamp[:n_param]:
-            st.refresh_weights(model)
+            changed = {i for i in range(n_param) if stamp[i] != st.stamp[i]}
+            st.refresh_weights(model, head=not changed <= st._torso_only, torso=not changed.isdisjoint(st._torso_only))
         st.stamp = stamp
     return st
 

@@ -70,3 +70,32 @@ def test_torso_field_follows_every_step(name):
     for step in range(3):
         assert all(torch.equal(a, b) for a, b in zip(run(model), run(copy.deepcopy(model)))), (name, step)
         opt.step()
+
+
+@pytest.mark.parametrize("which", ["torso", "head", "code", "both", "table"])
+def test_what_changed_is_repacked(which):
+    """Weights of the torso, of the head, an identity code, both, a table: a frame is bit for bit that of a copy that has packed nothing yet."""
+    from helpers import frame_inputs, sequence
+    from geneface_amd.radnerf_torso import RADNeRFTorso
+    hp, sd = model_fixture(True)
+    model = RADNeRFTorso(hp)
+    model.load_state_dict(sd, strict=True)
+    model = model.to(DEV).eval()
+    fi = frame_inputs(sequence(4, 32, 32), 1)
+    to = lambda t: t.to(DEV)      # noqa: E731
+    args = tuple(to(fi[k]) for k in ("rays_o", "rays_d", "cond", "bg_coords", "pose6"))
+
+    def run(m):
+        with torch.no_grad():
+            return m.render(*args, index=0, staged=False, bg_color=to(fi["bg"]), perturb=False, force_all_rays=True, render_impl="fused", **hp)["rgb_map"].clone()
+    names = {"torso": ["torso_canonicial_net.net.2.weight"], "head": ["sigma_net.net.1.weight"], "code": ["individual_embeddings", "torso_individual_codes"],
+             "both": ["torso_deform_net.net.0.weight", "color_net.net.0.weight"], "table": ["position_embedder.embeddings", "torso_embedder.embeddings"]}[which]
+    last = run(model)
+    for _ in range(2):
+        with torch.no_grad():
+            for n, p in model.named_parameters():
+                if n in names:
+                    p.mul_(1.1)
+        now = run(model)
+        assert torch.equal(now, run(copy.deepcopy(model))) and not torch.equal(now, last)
+        last = now
