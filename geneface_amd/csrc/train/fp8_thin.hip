@@ -6,7 +6,7 @@
 // avoid: a workgroup brings its 128 rows to 8 bits in LDS and multiplies them there.  The weight's codes stay in LDS for all its tiles.  Forward: x is
 // read once, y and (for the weight's gradient) x by columns are written.  Backward: dy is read once for both products; the weight's gradient is
 // added up in the registers of the workgroup over all its tiles, so that only a part per workgroup has to be joined.
-// Measured, 262221 rows, 96 -> 128, float32: forward 51-56 us with the weight's own quantisation (268 MB, 4.8-5.3 TB/s), backward 60-66 (293 MB, 4.4-4.9 TB/s), the join of its 512 parts 8.
+// Measured, 262221 rows, 96 -> 128, float32: forward 52-55 us with the weight's own quantisation (260 MB, 4.7-5.0 TB/s), backward 61-65 (285 MB, 4.4-4.7 TB/s), the join of its 512 parts 8.
 #include "../common.hpp"
 #include "fp8.hpp"
 #include "fp8_calls.hpp"

@@ -11,7 +11,8 @@ to zero.  Held as its root it does not overflow either: any finite gradient leav
 1.8e19 / sqrt(1 - beta2) leaves an infinite one, and its parameter stands still from then on).  A block that meets a gradient that is no finite number is none afterwards (all 128 values).
 
 Everything is done on the current stream of the tensors' device and may be captured into a graph; a graph keeps the addresses, and numbers given
-as Python numbers (`lr` as a one-element tensor on the device stays adjustable).
+as Python numbers (`lr` as a one-element tensor on the device stays adjustable).  A step raises the version counters of what it writes; a replay does not:
+whoever goes by them (the fused field's packed weights) needs `torch.autograd.graph.increment_version(params)` behind it.
 """
 import ctypes as C
 import math
