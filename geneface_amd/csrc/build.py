@@ -149,6 +149,8 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, varia
             print("linked", out)
     if host is not None and host.exception() is not None:      # the C ABI needs neither g++ nor Python's and torch's headers: lib.host() says what is missing when it is asked for
         sys.stderr.write(f"geneface_amd: {out} is built, the Python side of the training operators is not: {host.exception()}\n")
+        if os.path.exists(HOST_OUT):      # of older sources: it must not be loaded beside this library
+            os.remove(HOST_OUT)
     return out
 
 

@@ -65,3 +65,12 @@ def test_a_file_appears_when_it_is_whole(places):
     """While the compiler writes, nothing is there to be loaded."""
     _compiler(places / "g++", f'echo half > "$out"; [ -e {places / "host.so"} ] && echo early >&2 && exit 1; echo whole >> "$out"')
     assert build.build_host() == str(places / "host.so") and (places / "host.so").read_text() == "half\nwhole\n"
+
+
+def test_a_module_of_older_sources_is_not_kept_beside_a_new_library(places, capsys):
+    _compiler(places / "g++", 'echo made > "$out"')
+    build.build()
+    assert (places / "host.so").exists()
+    _compiler(places / "g++", "echo broken >&2; exit 1")
+    build.build(force=True)
+    assert "broken" in capsys.readouterr().err and (places / "lib.so").exists() and not (places / "host.so").exists()
