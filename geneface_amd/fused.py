@@ -10,6 +10,7 @@ Per-model state (packed weights, fold matrices, workspace) is built once and cac
 import ctypes as C
 import itertools
 import random
+import threading
 import weakref
 
 import numpy as np
@@ -166,7 +167,8 @@ class FusedState:
         self.stamp = _stamp(self._watch)
         # which of them only the torso's packs are made of
         self._torso_only = {i for i, (n, _) in enumerate(model.named_parameters()) if n.startswith(("torso", "head_color_weights_encoder"))}
-        _live.add(self)
+        with _live_lock:
+            _live.add(self)
 
     # ---- in-place weight updates (a training step, load_state_dict, a broadcast): repack on the device, no host round trip
     @staticmethod
@@ -367,7 +369,7 @@ def _watched_tensors(model):
 
 
 _untracked = itertools.count(-1, -1)
-_live = weakref.WeakSet()      # every FusedState in use
+_live, _live_lock = weakref.WeakSet(), threading.Lock()      # every FusedState in use
 
 
 def _after_optimizer_step(opt, args, kwargs):
@@ -375,7 +377,8 @@ def _after_optimizer_step(opt, args, kwargs):
     training step's forward pass would go on with the weights packed before the step."""
     if not any(g.get("fused") for g in opt.param_groups):
         return
-    watched = {id(t) for st in _live for t in st._watch}
+    with _live_lock:
+        watched = {id(t) for st in _live for t in st._watch}
     for g in opt.param_groups:
         if g.get("fused"):
             for p in g["params"]:
