@@ -90,7 +90,7 @@ class _linear_tall(torch.autograd.Function):
 
 def all_native(model):
     """Whether every MLP of a model computes in its layers' type, as the fused kernels do."""
-    return all(getattr(m, "precision", "native") == "native" for m in model.children())
+    return all(m.precision == "native" for m in model.children() if isinstance(m, MLP))
 
 
 class MLP(nn.Module):
